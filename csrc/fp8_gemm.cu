@@ -1,0 +1,494 @@
+// Block-scaled FP8 products on sm_100a tensor cores (tcgen05 + TMEM + TMA).
+//
+//   C[r, n] = sum over kb of sa[r, kb] * sb[n / 128, kb] * (A[r, kb] . B[g][n, kb])
+//
+// with e4m3 operands in blocks kb of 128 columns, one fp32 scale per 1 x 128
+// block of A (the FP8 dispatch's wire format) and per 128 x 128 block of B,
+// dense or grouped by expert with row counts on the device.
+//
+// The scales are any fp32 number, so they cannot ride along in the tensor core
+// (its block scales are powers of two).  The four K = 32 MMAs of one
+// 128-column block therefore go to a TMEM accumulator of their own; eight warps
+// drain it into registers with one fused multiply-add per element,
+// acc += (sa * sb) * partial, while the tensor core fills the other of two
+// accumulators.  Per block and SM: 128 x 256 x 128 multiply-adds are 512 tensor
+// cycles, the drain is 128 x 256 FMAs = 256 FP32-pipe cycles plus as many TMEM
+// read cycles, so it hides under the MMAs.
+//
+// Kernel shape (one CTA per SM, persistent over 128 x 256 tiles):
+//   warps 0..7   drain and epilogue: TMEM lane quadrant = warp % 4 (32 rows),
+//                columns [64 h, 64 h + 64) and [128 + 64 h, 128 + 64 h + 64) for
+//                h = warp / 4, so that with SwiGLU a thread owns matching gate
+//                and up columns; 128 fp32 sums in registers
+//   warp 8       TMA producer: 128 x 128-byte A tile + 256 x 128-byte B tile
+//   warp 9       TMEM owner and MMA issuer (warps 10 and 11 only fill its warpgroup)
+// Every wait is bounded; one that runs out sets the error word, and the CTA
+// drains its loads, frees its TMEM and leaves.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <mutex>
+
+#include "kiwi/ep/quant.cuh"
+#include "kiwi/gemm/fp8_gemm.hpp"
+#include "kiwi/gemm/group_table.cuh"
+#include "kiwi/gemm/grouped_gemm.hpp"
+#include "kiwi/gemm/tensor_map.hpp"
+#include "kiwi/sm100.cuh"
+
+namespace kiwi::gemm {
+
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kBN = 256;
+constexpr int kBK = 128;      // bytes = e4m3 elements = one scale block
+constexpr int kStages = 4;
+constexpr int kThreads = 384;  // two drain warpgroups; one with the producer, the MMA issuer and two idle warps
+constexpr int kDrainThreads = 256;
+// 128 sums and a 32-column TMEM load do not fit the 168 registers that 384
+// threads share evenly; the third warpgroup gives some of its own away.
+constexpr int kDrainRegs = 232, kIssueRegs = 40;
+static_assert(2 * kDrainRegs + kIssueRegs <= 3 * 168, "more registers than the CTA is launched with");
+
+enum Epi : int { kEpiStore = 0, kEpiSwiGLU = 1, kEpiSwiGLUQuant = 2 };
+
+struct Smem {
+    static constexpr int kABytes = kBM * kBK;
+    static constexpr int kBBytes = kBN * kBK;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kTableOffset = kStages * kStageBytes;
+    static constexpr int kAmaxOffset = kTableOffset + static_cast<int>(round_up(sizeof(GroupTable), 16));
+    static constexpr int kBarOffset = kAmaxOffset + 2 * 2 * kBM * 4;
+    static constexpr int kBytes = kBarOffset + 256 + 1024;  // barriers, TMEM slot, alignment slack
+};
+static_assert(Smem::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
+
+struct Params {
+    Fp8GemmArgs a;
+    int k_blocks;
+    int nb;  // scale blocks of B per group along n
+    uint32_t* error;
+};
+
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+
+/// acc += v * s on two fp32 lanes (one instruction).
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
+}
+
+__device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
+
+/// 64 consecutive columns of one row as bf16, `cols` of them inside the matrix.
+__device__ __forceinline__ void store_row64(__nv_bfloat16* dst, const float (&v)[64], int cols, bool vec) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = v[8 * j + i];
+        if (vec && 8 * j + 8 <= cols) {
+            *reinterpret_cast<uint4*>(dst + 8 * j) = ep::f32x8_to_bf16(f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (8 * j + i < cols) dst[8 * j + i] = __float2bfloat16_rn(f[i]);
+            }
+        }
+    }
+}
+
+template <int EPI>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                    const __grid_constant__ Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    GroupTable& table = *reinterpret_cast<GroupTable*>(smem + Smem::kTableOffset);
+    float* s_amax = reinterpret_cast<float*>(smem + Smem::kAmaxOffset);  // [tile parity][column half][row]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Smem::kBarOffset);
+    uint64_t* empty = full + kStages;
+    uint64_t* tmem_full = empty + kStages;
+    uint64_t* tmem_empty = tmem_full + 2;
+    uint64_t* amax_bar = tmem_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(amax_bar + 1);
+    __shared__ int s_abort;
+
+    const int warp = threadIdx.x / 32;
+    const int lane = threadIdx.x & 31;
+    const int groups = p.a.num_groups;
+    const int n_tiles = (p.a.n + kBN - 1) / kBN;
+    const int k_blocks = p.k_blocks;
+
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int s = 0; s < kStages; ++s) {
+            sm100::mbar_init(&full[s], 1);
+            sm100::mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            sm100::mbar_init(&tmem_full[i], 1);
+            sm100::mbar_init(&tmem_empty[i], kDrainThreads / 32);
+        }
+        sm100::mbar_init(amax_bar, kDrainThreads);
+        sm100::fence_mbar_init();
+    }
+    if (warp == 8 && lane == 0) {
+        sm100::tma_prefetch_desc(&tmap_a);
+        sm100::tma_prefetch_desc(&tmap_b);
+    }
+    if (warp == 9) sm100::tmem_alloc(tmem_slot, 2 * kBN);
+    build_group_table(table, p.a.counts, groups, p.a.rows, kBM, n_tiles, p.error);
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = table.tiles[groups];
+
+    auto aborted = [&]() { return *reinterpret_cast<volatile int*>(&s_abort) != 0; };
+    auto fail = [&]() {
+        *reinterpret_cast<volatile int*>(&s_abort) = 1;
+        atomicOr(p.error, kGemmTimeout);
+    };
+
+    if (warp >= 8) {
+        sm100::reg_dec<kIssueRegs>();
+        if (warp == 8 && lane == 0) {
+            uint32_t issued = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
+                int g, mt, nt;
+                find_tile(table, groups, n_tiles, tile, g, mt, nt);
+                const int row0 = table.off[g] + mt * kBM;
+                const int brow0 = g * p.a.n + nt * kBN;
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    const uint32_t stage = issued % kStages;
+                    if (!sm100::mbar_wait(&empty[stage], ((issued / kStages) & 1) ^ 1)) {
+                        fail();
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sa = smem + stage * Smem::kStageBytes;
+                    sm100::mbar_arrive_expect_tx(&full[stage], Smem::kStageBytes);
+                    sm100::tma_load_2d(sa, &tmap_a, &full[stage], kb * kBK, row0);
+                    sm100::tma_load_2d(sa + Smem::kABytes, &tmap_b, &full[stage], kb * kBK, brow0);
+                    ++issued;
+                }
+            }
+            // No load may still be in flight when this CTA's shared memory goes away.
+            for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
+                if (!sm100::mbar_wait(&full[i % kStages], (i / kStages) & 1)) fail();
+            }
+        } else if (warp == 9 && lane == 0) {
+            const uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kBN);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
+                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                    const uint32_t stage = it % kStages;
+                    const uint32_t buf = it & 1;
+                    if (!sm100::mbar_wait(&tmem_empty[buf], ((it >> 1) & 1) ^ 1) ||
+                        !sm100::mbar_wait(&full[stage], (it / kStages) & 1)) {
+                        fail();
+                        ok = false;
+                        break;
+                    }
+                    sm100::tc_fence_after();
+                    uint8_t* sa = smem + stage * Smem::kStageBytes;
+                    const uint64_t ad = sm100::sw128_kmajor_desc(sa);
+                    const uint64_t bd = sm100::sw128_kmajor_desc(sa + Smem::kABytes);
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 32; ++kk) {  // 32 bytes of K = 2 descriptor units a step
+                        sm100::mma_f8(tmem_base + buf * kBN, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                    }
+                    sm100::mma_commit(&empty[stage]);
+                    sm100::mma_commit(&tmem_full[buf]);
+                }
+            }
+            // Nor may an MMA still write the TMEM that is freed below.
+            if (it > 0 && !sm100::mbar_wait(&tmem_full[(it - 1) & 1], ((it - 1) >> 1) & 1)) fail();
+        }
+    } else {
+        sm100::reg_inc<kDrainRegs>();
+        const int q = warp & 3;
+        const int half = warp >> 2;
+        const int row_in_tile = q * 32 + lane;
+        const bool vec = p.a.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.a.c) % 16 == 0;
+        uint32_t it = 0;
+        uint32_t n_done = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x, ++n_done) {
+            int g, mt, nt;
+            find_tile(table, groups, n_tiles, tile, g, mt, nt);
+            const int64_t row = static_cast<int64_t>(table.off[g]) + mt * kBM + row_in_tile;
+            const bool valid = row < table.off[g + 1];
+            const float* sa = p.a.a_scale + (valid ? row : 0) * p.a.a_scale_stride;
+            const int bb = nt * 2;
+            const float* sb0 = p.a.b_scale + (static_cast<int64_t>(g) * p.nb + bb) * k_blocks;
+            const float* sb1 = bb + 1 < p.nb ? sb0 + k_blocks : sb0;
+            float a_next = __ldg(sa), b0_next = __ldg(sb0), b1_next = __ldg(sb1);
+            uint64_t acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0;
+#pragma unroll 1
+            for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                const float s0 = a_next * b0_next, s1 = a_next * b1_next;
+                if (kb + 1 < k_blocks) {  // the next block's scales travel while this one's MMAs run
+                    a_next = __ldg(sa + kb + 1);
+                    b0_next = __ldg(sb0 + kb + 1);
+                    b1_next = __ldg(sb1 + kb + 1);
+                }
+                const uint32_t buf = it & 1;
+                if (!sm100::mbar_wait(&tmem_full[buf], (it >> 1) & 1)) {
+                    fail();
+                    ok = false;
+                    break;
+                }
+                sm100::tc_fence_after();
+                const uint32_t taddr =
+                    tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + static_cast<uint32_t>(half * 64);
+                const uint64_t ss0 = pack2(s0, s0), ss1 = pack2(s1, s1);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float v[32];
+                    sm100::tmem_ld_32cols(taddr + (c >> 1) * 128 + (c & 1) * 32, v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], pack2(v[2 * i], v[2 * i + 1]), c < 2 ? ss0 : ss1);
+                }
+                sm100::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) sm100::mbar_arrive(&tmem_empty[buf]);
+            }
+            if (!ok) break;
+            if constexpr (EPI == kEpiStore) {
+                const float scale = valid && p.a.row_scale ? __ldg(p.a.row_scale + row) : 1.0f;
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    float v[64];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float2 f = unpack2(acc[part * 32 + i]);
+                        v[2 * i] = f.x * scale;
+                        v[2 * i + 1] = f.y * scale;
+                    }
+                    const int col = nt * kBN + part * 128 + half * 64;
+                    if (valid && col < p.a.n) store_row64(p.a.c + row * p.a.ldc + col, v, p.a.n - col, vec);
+                }
+            } else {
+                float h[64];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float2 gt = unpack2(acc[i]);
+                    const float2 up = unpack2(acc[32 + i]);
+                    h[2 * i] = silu(gt.x) * up.x;
+                    h[2 * i + 1] = silu(gt.y) * up.y;
+                }
+                const int col = nt * (kBN / 2) + half * 64;
+                if constexpr (EPI == kEpiSwiGLU) {
+                    const float scale = valid && p.a.row_scale ? __ldg(p.a.row_scale + row) : 1.0f;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) h[i] *= scale;
+                    if (valid) store_row64(p.a.c + row * p.a.ldc + col, h, 64, vec);
+                } else {
+                    // The tile's 128 hidden columns are one scale block; its other 64
+                    // columns are in the thread of the same row in the other four warps.
+                    float amax = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) amax = fmaxf(amax, fabsf(h[i]));
+                    float* slot = s_amax + (n_done & 1) * 2 * kBM;
+                    slot[half * kBM + row_in_tile] = amax;
+                    sm100::mbar_arrive(amax_bar);
+                    if (!sm100::mbar_wait(amax_bar, n_done & 1)) {
+                        fail();
+                        break;
+                    }
+                    amax = fmaxf(amax, slot[(half ^ 1) * kBM + row_in_tile]);
+                    const float scale = amax > 0.f ? amax / ep::kFp8Max : 1.0f;
+                    const float inv = amax > 0.f ? ep::kFp8Max / amax : 0.f;
+                    if (valid) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint32_t lo = __nv_cvt_float2_to_fp8x2(
+                                make_float2(h[4 * i] * inv, h[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                            const uint32_t hi = __nv_cvt_float2_to_fp8x2(
+                                make_float2(h[4 * i + 2] * inv, h[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+                            w[i] = lo | (hi << 16);
+                        }
+                        uint4* dst = reinterpret_cast<uint4*>(p.a.codes + row * (p.a.n / 2) + col);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                        if (half == 0) p.a.scales[row * (p.a.n / kBN) + nt] = scale;
+                    }
+                }
+            }
+        }
+        if (p.a.zero_tail) {
+            const int cols = EPI == kEpiStore ? p.a.n : p.a.n / 2;
+            for (int64_t r = table.off[groups] + static_cast<int64_t>(blockIdx.x); r < p.a.rows; r += gridDim.x) {
+                if constexpr (EPI == kEpiSwiGLUQuant) {
+                    for (int c = threadIdx.x * 16; c < cols; c += kDrainThreads * 16) {
+                        *reinterpret_cast<uint4*>(p.a.codes + r * cols + c) = make_uint4(0, 0, 0, 0);
+                    }
+                    for (int c = threadIdx.x; c < cols / 128; c += kDrainThreads) p.a.scales[r * (cols / 128) + c] = 1.0f;
+                } else {
+                    for (int c = threadIdx.x; c < cols; c += kDrainThreads) p.a.c[r * p.a.ldc + c] = __float2bfloat16_rn(0.f);
+                }
+            }
+        }
+    }
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    if (warp == 9) sm100::tmem_dealloc(tmem_base, 2 * kBN);
+}
+
+// ---------------------------------------------------------------------------
+// 128 x 128 block quantisation of weights: one CTA per block, which stays in
+// registers between its maximum and its conversion (64 bf16 values a thread:
+// 8 rows of 8 columns), so w is read once.  Bound by memory; a one-time cost
+// when weights are loaded.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) quant_fp8_blocks_kernel(const __nv_bfloat16* __restrict__ w, int64_t ld,
+                                                               int64_t rows, int64_t cols, int64_t col_blocks,
+                                                               bool vec, uint8_t* __restrict__ codes,
+                                                               float* __restrict__ scales) {
+    __shared__ float s_max[8];
+    const int64_t rb = blockIdx.x / col_blocks, cb = blockIdx.x % col_blocks;
+    const int64_t c = cb * 128 + (threadIdx.x & 15) * 8;
+    const int64_t r0 = rb * 128 + (threadIdx.x >> 4);
+    const bool whole = vec && c + 8 <= cols;
+    uint4 in[8];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t r = r0 + 16 * i;
+        in[i] = make_uint4(0, 0, 0, 0);
+        if (r < rows) {
+            if (whole) {
+                in[i] = *reinterpret_cast<const uint4*>(w + r * ld + c);
+            } else {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = c + j < cols ? __bfloat162float(w[r * ld + c + j]) : 0.f;
+                in[i] = ep::f32x8_to_bf16(f);
+            }
+        }
+        float f[8];
+        ep::bf16x8_to_f32(in[i], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(f[j]));
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, s_max[i]);
+    const float scale = amax > 0.f ? amax / ep::kFp8Max : 1.0f;
+    const float inv = amax > 0.f ? ep::kFp8Max / amax : 0.f;
+    if (threadIdx.x == 0) scales[blockIdx.x] = scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t r = r0 + 16 * i;
+        if (r >= rows) continue;
+        float f[8];
+        ep::bf16x8_to_f32(in[i], f);
+        uint8_t q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = __nv_cvt_float_to_fp8(f[j] * inv, __NV_SATFINITE, __NV_E4M3);
+        uint8_t* dst = codes + r * cols + c;
+        if (c + 8 <= cols && cols % 8 == 0) {
+            uint2 o;
+            o.x = q[0] | (q[1] << 8) | (q[2] << 16) | (static_cast<uint32_t>(q[3]) << 24);
+            o.y = q[4] | (q[5] << 8) | (q[6] << 16) | (static_cast<uint32_t>(q[7]) << 24);
+            *reinterpret_cast<uint2*>(dst) = o;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (c + j < cols) dst[j] = q[j];
+            }
+        }
+    }
+}
+
+__device__ uint32_t g_error;
+
+template <int EPI>
+void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int grid, cudaStream_t stream) {
+    static std::atomic<uint64_t> attr{0};
+    raise_smem_limit(reinterpret_cast<const void*>(fp8_gemm_kernel<EPI>), Smem::kBytes, attr);
+    fp8_gemm_kernel<EPI><<<grid, kThreads, Smem::kBytes, stream>>>(ta, tb, p);
+    KIWI_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace
+
+uint32_t* gemm_error_word() {
+    static std::mutex mu;
+    static uint32_t* ptr[64] = {};
+    int dev = 0;
+    KIWI_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) throw kiwi::error("gemm_error_word: device index beyond 64");
+    std::lock_guard<std::mutex> lock(mu);
+    if (!ptr[dev]) {
+        void* q = nullptr;
+        KIWI_CUDA_CHECK(cudaGetSymbolAddress(&q, g_error));
+        ptr[dev] = static_cast<uint32_t*>(q);
+    }
+    return ptr[dev];
+}
+
+void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream) {
+    if (args.num_groups < 1 || args.num_groups > kMaxGroups) throw kiwi::error("fp8_gemm: 1..1024 groups");
+    if (args.n < 1 || args.k < 16 || args.k % 16 != 0) throw kiwi::error("fp8_gemm: K must be a positive multiple of 16");
+    if (args.num_groups > 1 && args.n % 128 != 0) throw kiwi::error("fp8_gemm: grouped N must be a multiple of 128");
+    if (args.swiglu && args.n % kBN != 0) throw kiwi::error("fp8_gemm: SwiGLU needs N to be a multiple of 256");
+    if (args.codes && !args.swiglu) throw kiwi::error("fp8_gemm: FP8 output needs swiglu");
+    if (args.rows < 0 || args.rows > INT32_MAX - kBM ||
+        static_cast<int64_t>(args.num_groups) * args.n > INT32_MAX - kBN) {
+        throw kiwi::error("fp8_gemm: more than 2^31 rows");
+    }
+    if (args.rows == 0) return;
+    Params p{};
+    p.a = args;
+    p.k_blocks = (args.k + kBK - 1) / kBK;
+    p.nb = (args.n + 127) / 128;
+    p.error = gemm_error_word();
+    const CUtensorMap ta = make_tmap_2d(args.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, args.rows, args.k, args.lda, kBM, kBK);
+    const CUtensorMap tb = make_tmap_2d(args.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1,
+                                        static_cast<uint64_t>(args.num_groups) * args.n, args.k, args.ldb, kBN, kBK);
+    // At most this many tiles, however the rows fall into groups.
+    const int64_t n_tiles = (args.n + kBN - 1) / kBN;
+    const int64_t most = ((args.rows + kBM - 1) / kBM + (args.counts ? args.num_groups : 0)) * n_tiles;
+    const int sms = num_sms();
+    const int grid = static_cast<int>(most < sms ? most : sms);
+    if (!args.swiglu) launch<kEpiStore>(ta, tb, p, grid, stream);
+    else if (!args.codes) launch<kEpiSwiGLU>(ta, tb, p, grid, stream);
+    else launch<kEpiSwiGLUQuant>(ta, tb, p, grid, stream);
+}
+
+void quant_fp8_blocks(const __nv_bfloat16* w, int64_t ld, int64_t rows, int64_t cols, uint8_t* codes, float* scales,
+                      cudaStream_t stream) {
+    if (rows <= 0 || cols <= 0) return;
+    const int64_t cb = (cols + 127) / 128, blocks = (rows + 127) / 128 * cb;
+    if (blocks > INT32_MAX) throw kiwi::error("quant_fp8_blocks: matrix too large");
+    quant_fp8_blocks_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+        w, ld, rows, cols, cb, ld % 8 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0, codes, scales);
+    KIWI_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace kiwi::gemm

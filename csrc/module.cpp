@@ -27,6 +27,7 @@ using namespace kiwi;
 void register_p2p(py::module_& m);
 void register_ep(py::module_& m);
 void register_ops(py::module_& m);
+void register_expert_ops(py::module_& m);
 
 namespace {
 
@@ -737,4 +738,5 @@ PYBIND11_MODULE(_C, m) {
     register_p2p(m);
     register_ep(m);
     register_ops(m);
+    register_expert_ops(m);
 }

@@ -1,0 +1,119 @@
+// SwiGLU between the experts' two products, with routing weights, and its gradients.
+//
+//   h = s * a * u                      a = g * sig(g)
+//   du = dh * s * a
+//   dg = dh * s * u * sig(g) * (1 + g * (1 - sig(g)))
+//   ds = sum over the row of dh * a * u
+//
+// g and u are the gate and up columns of a row of y, in blocks of 128 each (the
+// layout of the grouped products).  All arithmetic is fp32; each result is
+// rounded once to bf16, ds is summed and kept in fp32 in an order that depends
+// on nothing but the row's length.
+//
+// Bound by memory: forward reads 4 F bytes a row and writes 2 F, backward reads
+// 6 F and writes 4 F.  One warp takes a row, 256 hidden columns a step, eight
+// columns (one 16-byte access of each operand) a lane.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "kiwi/common.hpp"
+#include "kiwi/ep/quant.cuh"
+#include "kiwi/ops/swiglu.hpp"
+
+namespace kiwi::ops {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRowsPerBlock = kThreads / 32;
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+/// Column of y that holds the gate of hidden column j (its up column is 128 further).
+__device__ __forceinline__ int gate_col(int j) { return (j >> 7) * 256 + (j & 127); }
+
+__global__ void __launch_bounds__(kThreads) swiglu_forward_kernel(const __nv_bfloat16* __restrict__ y, int64_t ldy,
+                                                                  const float* __restrict__ row_scale,
+                                                                  __nv_bfloat16* __restrict__ h, int64_t rows,
+                                                                  int ffn) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const float s = row_scale ? __ldg(row_scale + r) : 1.0f;
+    const __nv_bfloat16* yr = y + r * ldy;
+    __nv_bfloat16* hr = h + r * ffn;
+#pragma unroll 4
+    for (int j = (threadIdx.x & 31) * 8; j < ffn; j += 256) {
+        const int c = gate_col(j);
+        float g[8], u[8], o[8];
+        ep::bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(yr + c)), g);
+        ep::bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(yr + c + 128)), u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = g[i] * sigmoid(g[i]) * u[i] * s;
+        *reinterpret_cast<uint4*>(hr + j) = ep::f32x8_to_bf16(o);
+    }
+}
+
+__global__ void __launch_bounds__(kThreads)
+    swiglu_backward_kernel(const __nv_bfloat16* __restrict__ dh, int64_t lddh, const __nv_bfloat16* __restrict__ y,
+                           int64_t ldy, const float* __restrict__ row_scale, __nv_bfloat16* __restrict__ dy,
+                           float* __restrict__ drow_scale, int64_t rows, int ffn) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const float s = row_scale ? __ldg(row_scale + r) : 1.0f;
+    const __nv_bfloat16* yr = y + r * ldy;
+    const __nv_bfloat16* dhr = dh + r * lddh;
+    __nv_bfloat16* dyr = dy + r * 2 * ffn;
+    float sum = 0.f;
+#pragma unroll 2
+    for (int j = (threadIdx.x & 31) * 8; j < ffn; j += 256) {
+        const int c = gate_col(j);
+        float g[8], u[8], d[8], dg[8], du[8];
+        ep::bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(yr + c)), g);
+        ep::bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(yr + c + 128)), u);
+        ep::bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(dhr + j)), d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float sig = sigmoid(g[i]);
+            const float a = g[i] * sig;
+            const float ds = d[i] * s;
+            sum += d[i] * a * u[i];
+            du[i] = ds * a;
+            dg[i] = ds * u[i] * sig * (1.0f + g[i] * (1.0f - sig));
+        }
+        *reinterpret_cast<uint4*>(dyr + c) = ep::f32x8_to_bf16(dg);
+        *reinterpret_cast<uint4*>(dyr + c + 128) = ep::f32x8_to_bf16(du);
+    }
+    if (drow_scale) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if ((threadIdx.x & 31) == 0) drow_scale[r] = sum;
+    }
+}
+
+unsigned blocks_for(int64_t rows) {
+    const int64_t b = (rows + kRowsPerBlock - 1) / kRowsPerBlock;
+    if (b > INT32_MAX) throw kiwi::error("swiglu: too many rows");
+    return static_cast<unsigned>(b);
+}
+
+}  // namespace
+
+void swiglu_forward(const __nv_bfloat16* y, int64_t ldy, const float* row_scale, __nv_bfloat16* h, int64_t rows,
+                    int ffn, cudaStream_t s) {
+    if (rows <= 0) return;
+    swiglu_forward_kernel<<<blocks_for(rows), kThreads, 0, s>>>(y, ldy, row_scale, h, rows, ffn);
+    KIWI_CUDA_CHECK(cudaGetLastError());
+}
+
+void swiglu_backward(const __nv_bfloat16* dh, int64_t lddh, const __nv_bfloat16* y, int64_t ldy,
+                     const float* row_scale, __nv_bfloat16* dy, float* drow_scale, int64_t rows, int ffn,
+                     cudaStream_t s) {
+    if (rows <= 0) return;
+    swiglu_backward_kernel<<<blocks_for(rows), kThreads, 0, s>>>(dh, lddh, y, ldy, row_scale, dy, drow_scale, rows,
+                                                                 ffn);
+    KIWI_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace kiwi::ops

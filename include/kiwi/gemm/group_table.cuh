@@ -1,0 +1,125 @@
+// The tile schedule of a grouped product, built by every CTA in its own shared
+// memory from the groups' row counts on the device: no schedule launch before
+// the product, no host synchronisation, no workspace that two launches could
+// share.  One read of at most 4 KB of counts and a warp scan cost about a
+// microsecond at 1024 groups and less than the barrier set-up at 32.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "kiwi/common.hpp"
+
+namespace kiwi::gemm {
+
+inline constexpr int kMaxGroups = 1024;
+
+// Error bits of the products' device error word (see gemm_error_word()).
+inline constexpr uint32_t kGemmTimeout = 1u;   // a bounded wait ran out: the output is incomplete
+inline constexpr uint32_t kGemmCounts = 2u;    // a negative count, or counts whose sum exceeds the rows
+
+#if defined(__CUDACC__)
+
+/// off[g] .. off[g + 1] are group g's rows; tiles[g] its first tile.
+struct GroupTable {
+    int32_t off[kMaxGroups + 1];
+    int32_t tiles[kMaxGroups + 1];
+};
+
+/// Whole CTA; ends with a __syncthreads().  Counts are clamped to what `rows`
+/// can hold, so every offset is a valid row whatever the counts are (a bad
+/// count sets kGemmCounts in *error).  counts == nullptr: one group of all rows.
+/// `bm` rows and `n_tiles` column tiles make a tile.
+__device__ __forceinline__ void build_group_table(GroupTable& t, const int32_t* counts, int groups, int64_t rows,
+                                                  int bm, int n_tiles, uint32_t* error) {
+    if (counts == nullptr) {
+        if (threadIdx.x == 0) {
+            t.off[0] = 0;
+            t.off[1] = static_cast<int32_t>(rows);
+            t.tiles[0] = 0;
+            t.tiles[1] = static_cast<int32_t>((rows + bm - 1) / bm) * n_tiles;
+        }
+        __syncthreads();
+        return;
+    }
+    bool bad = false;
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+        int32_t c = __ldg(&counts[g]);
+        if (c < 0) {
+            bad = true;
+            c = 0;
+        }
+        t.off[g + 1] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        const int per = (groups + 31) / 32;
+        const int g0 = lane * per;
+        const int g1 = g0 + per < groups ? g0 + per : groups;
+        int64_t sum = 0;
+        for (int g = g0; g < g1; ++g) sum += t.off[g + 1];
+        int64_t incl = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += y;
+        }
+        int64_t at = incl - sum;
+        int32_t tl = 0;  // this lane's tiles
+        int64_t pos = at;
+        for (int g = g0; g < g1; ++g) {
+            const int64_t end = pos + t.off[g + 1];
+            const int64_t c = (end < rows ? end : rows) - (pos < rows ? pos : rows);
+            tl += static_cast<int32_t>((c + bm - 1) / bm);
+            pos = end;
+        }
+        int32_t tincl = tl;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int32_t y = __shfl_up_sync(0xffffffffu, tincl, d);
+            if (lane >= d) tincl += y;
+        }
+        int32_t tile = (tincl - tl) * n_tiles;
+        pos = at;
+        for (int g = g0; g < g1; ++g) {
+            const int64_t first = pos < rows ? pos : rows;
+            const int64_t end = pos + t.off[g + 1];
+            const int64_t last = end < rows ? end : rows;
+            if (end > rows) bad = true;
+            tile += static_cast<int32_t>((last - first + bm - 1) / bm) * n_tiles;
+            t.off[g + 1] = static_cast<int32_t>(last);  // this lane alone reads and writes its groups' entries
+            t.tiles[g + 1] = tile;
+            pos = end;
+        }
+        if (lane == 0) {
+            t.off[0] = 0;
+            t.tiles[0] = 0;
+        }
+    }
+    if (bad && error && blockIdx.x == 0) atomicOr(error, kGemmCounts);
+    __syncthreads();
+}
+
+/// Group, row block and column block of a tile.  The column block is outermost
+/// within a group: the row blocks that share one weight tile are neighbours in
+/// the schedule, run at the same time and read it from L2.
+__device__ __forceinline__ void find_tile(const GroupTable& t, int groups, int n_tiles, int tile, int& g, int& mt,
+                                          int& nt) {
+    int lo = 0, hi = groups - 1;
+    while (lo < hi) {  // first g with tiles[g + 1] > tile
+        const int mid = (lo + hi) >> 1;
+        if (t.tiles[mid + 1] > tile) hi = mid;
+        else lo = mid + 1;
+    }
+    g = lo;
+    const int local = tile - t.tiles[g];
+    const int m_tiles = (t.tiles[g + 1] - t.tiles[g]) / n_tiles;
+    nt = local / m_tiles;
+    mt = local - nt * m_tiles;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace kiwi::gemm

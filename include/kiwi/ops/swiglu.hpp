@@ -1,0 +1,23 @@
+// Host API of SwiGLU and its gradient (csrc/swiglu_gpu.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace kiwi::ops {
+
+/// h[r, j] = row_scale[r] * silu(gate) * up for y [rows, 2 * ffn] (row stride ldy,
+/// a multiple of 8, 16-byte aligned) whose columns come in blocks of 128 gate and
+/// 128 up columns; h [rows, ffn] contiguous.  row_scale may be null (1).
+void swiglu_forward(const __nv_bfloat16* y, int64_t ldy, const float* row_scale, __nv_bfloat16* h, int64_t rows,
+                    int ffn, cudaStream_t s);
+
+/// Gradients of swiglu_forward: dy [rows, 2 * ffn] contiguous and, when
+/// drow_scale is not null, drow_scale [rows].
+void swiglu_backward(const __nv_bfloat16* dh, int64_t lddh, const __nv_bfloat16* y, int64_t ldy,
+                     const float* row_scale, __nv_bfloat16* dy, float* drow_scale, int64_t rows, int ffn,
+                     cudaStream_t s);
+
+}  // namespace kiwi::ops

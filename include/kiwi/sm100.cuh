@@ -153,6 +153,26 @@ KIWI_DEV uint64_t sw64_kmajor_desc(const void* smem_tile) {
     return d;
 }
 
+/// Descriptor of an MN-major, 128-byte-swizzled bf16 operand: boxes of 64 K
+/// rows x 64 MN columns (128 bytes a row) as a SWIZZLE_128B TMA load writes
+/// them, one box of 8 KB per 64 MN columns.  The canonical MN-major layout
+/// Swizzle<3,4,3> o ((8,8,m),(8,k)):((1,8,LBO),(64,SBO)) in elements: 8-row K
+/// groups 1024 bytes apart (SBO), 64-column MN atoms one box apart (LBO).
+KIWI_DEV uint64_t sw128_mnmajor_desc(const void* smem_tile) {
+    const uint64_t addr = smem_addr(smem_tile);
+    uint64_t d = 0;
+    d |= (addr >> 4) & 0x3FFFull;
+    d |= static_cast<uint64_t>(8192 >> 4) << 16;   // LBO between 64-column atoms
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;   // SBO between 8-row groups
+    d |= static_cast<uint64_t>(1) << 46;           // descriptor version (sm100)
+    d |= static_cast<uint64_t>(2) << 61;           // SWIZZLE_128B
+    return d;
+}
+
+/// Instruction descriptor bits: the A / B operand is MN-major.
+inline constexpr uint32_t kIdescAMn = 1u << 15;
+inline constexpr uint32_t kIdescBMn = 1u << 16;
+
 /// Descriptor of a K-major tile whose rows hold BK bf16 (64: 128-byte swizzle,
 /// 32: 64-byte swizzle; 128: two 128-byte-swizzled 64-column sub-tiles one after
 /// the other, the descriptor of the first).
@@ -170,6 +190,35 @@ KIWI_HD constexpr uint32_t idesc_bf16_f32(uint32_t m, uint32_t n) {
            | (1u << 10)         // B format: BF16
            | ((n >> 3) << 17)   // N >> 3
            | ((m >> 4) << 24);  // M >> 4
+}
+
+/// Instruction descriptor, kind::f8f6f4 with E4M3 A/B, FP32 accumulate, both K-major.
+KIWI_HD constexpr uint32_t idesc_e4m3_f32(uint32_t m, uint32_t n) {
+    return (1u << 4)            // D format: F32
+           | (0u << 7)          // A format: E4M3
+           | (0u << 10)         // B format: E4M3
+           | ((n >> 3) << 17)   // N >> 3
+           | ((m >> 4) << 24);  // M >> 4
+}
+
+/// D[tmem] (+)= A[smem] * B[smem]^T in 8-bit floating point (K = 32), issued by one thread.
+KIWI_DEV void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+/// mma_f8 over the tiles of a CTA pair (M = 256 across the pair).
+KIWI_DEV void mma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
 /// D[tmem] (+)= A[smem] * B[smem]^T, issued by one thread.
@@ -210,6 +259,18 @@ KIWI_DEV void tmem_ld_32cols(uint32_t taddr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+
+// ---- registers between warpgroups (whole warpgroup; the shares must not exceed the launch's total) ----
+
+template <int N>
+KIWI_DEV void reg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int N>
+KIWI_DEV void reg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 // ---- clusters of two CTAs (2-SM UMMA) ----
 
