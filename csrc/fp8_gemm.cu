@@ -30,6 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cstdlib>
 #include <mutex>
 
 #include "kiwi/ep/quant.cuh"
@@ -46,7 +47,6 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kBN = 256;
 constexpr int kBK = 128;      // bytes = e4m3 elements = one scale block
-constexpr int kStages = 4;
 constexpr int kThreads = 384;  // two drain warpgroups; one with the producer, the MMA issuer and two idle warps
 constexpr int kDrainThreads = 256;
 // 128 sums and a 32-column TMEM load do not fit the 168 registers that 384
@@ -56,16 +56,18 @@ static_assert(2 * kDrainRegs + kIssueRegs <= 3 * 168, "more registers than the C
 
 enum Epi : int { kEpiStore = 0, kEpiSwiGLU = 1, kEpiSwiGLUQuant = 2 };
 
+template <bool PAIR>
 struct Smem {
+    static constexpr int kStages = PAIR ? 6 : 4;
     static constexpr int kABytes = kBM * kBK;
-    static constexpr int kBBytes = kBN * kBK;
+    static constexpr int kBBytes = (PAIR ? kBN / 2 : kBN) * kBK;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kTableOffset = kStages * kStageBytes;
     static constexpr int kAmaxOffset = kTableOffset + static_cast<int>(round_up(sizeof(GroupTable), 16));
     static constexpr int kBarOffset = kAmaxOffset + 2 * 2 * kBM * 4;
     static constexpr int kBytes = kBarOffset + 256 + 1024;  // barriers, TMEM slot, alignment slack
 };
-static_assert(Smem::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
+static_assert(Smem<false>::kBytes <= 227 * 1024 && Smem<true>::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
 
 struct Params {
     Fp8GemmArgs a;
@@ -77,6 +79,12 @@ struct Params {
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
     return r;
 }
 
@@ -111,37 +119,40 @@ __device__ __forceinline__ void store_row64(__nv_bfloat16* dst, const float (&v)
     }
 }
 
-template <int EPI>
+template <int EPI, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const __grid_constant__ Params p) {
+    using S = Smem<PAIR>;
+    constexpr int kStages = S::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    GroupTable& table = *reinterpret_cast<GroupTable*>(smem + Smem::kTableOffset);
-    float* s_amax = reinterpret_cast<float*>(smem + Smem::kAmaxOffset);  // [tile parity][column half][row]
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Smem::kBarOffset);
-    uint64_t* empty = full + kStages;
-    uint64_t* tmem_full = empty + kStages;
-    uint64_t* tmem_empty = tmem_full + 2;
+    GroupTable& table = *reinterpret_cast<GroupTable*>(smem + S::kTableOffset);
+    float* s_amax = reinterpret_cast<float*>(smem + S::kAmaxOffset);  // [tile parity][column half][row]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBarOffset);
+    uint64_t* done = full + kStages;  // a stage's MMAs: its operands may be overwritten, its partial sums drained
+    uint64_t* tmem_empty = done + kStages;
     uint64_t* amax_bar = tmem_empty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(amax_bar + 1);
     __shared__ int s_abort;
 
-    const int warp = threadIdx.x / 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform: the roles' addresses stay in uniform registers
     const int lane = threadIdx.x & 31;
     const int groups = p.a.num_groups;
     const int n_tiles = (p.a.n + kBN - 1) / kBN;
     const int k_blocks = p.k_blocks;
+    const int crank = PAIR ? static_cast<int>(sm100::cluster_ctarank()) : 0;
+    const int first_tile = PAIR ? blockIdx.x / 2 : blockIdx.x;
+    const int tile_step = PAIR ? gridDim.x / 2 : gridDim.x;
 
     if (threadIdx.x == 0) {
         s_abort = 0;
         for (int s = 0; s < kStages; ++s) {
             sm100::mbar_init(&full[s], 1);
-            sm100::mbar_init(&empty[s], 1);
+            sm100::mbar_init(&done[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            sm100::mbar_init(&tmem_full[i], 1);
-            sm100::mbar_init(&tmem_empty[i], kDrainThreads / 32);
+            sm100::mbar_init(&tmem_empty[i], (PAIR ? 2 : 1) * kDrainThreads / 32);
         }
         sm100::mbar_init(amax_bar, kDrainThreads);
         sm100::fence_mbar_init();
@@ -150,10 +161,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::tma_prefetch_desc(&tmap_a);
         sm100::tma_prefetch_desc(&tmap_b);
     }
-    if (warp == 9) sm100::tmem_alloc(tmem_slot, 2 * kBN);
-    build_group_table(table, p.a.counts, groups, p.a.rows, kBM, n_tiles, p.error);
+    if (warp == 9) {
+        if constexpr (PAIR) sm100::tmem_alloc_pair(tmem_slot, 2 * kBN);
+        else sm100::tmem_alloc(tmem_slot, 2 * kBN);
+    }
+    build_group_table(table, p.a.counts, groups, p.a.rows, PAIR ? 2 * kBM : kBM, n_tiles, p.error);
     sm100::tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) sm100::cluster_sync();  // both CTAs' barriers exist before any arrival from the other
     sm100::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = table.tiles[groups];
@@ -169,57 +184,76 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 8 && lane == 0) {
             uint32_t issued = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
+            for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
                 int g, mt, nt;
                 find_tile(table, groups, n_tiles, tile, g, mt, nt);
-                const int row0 = table.off[g] + mt * kBM;
-                const int brow0 = g * p.a.n + nt * kBN;
+                const int row0 = table.off[g] + (PAIR ? 2 * mt + crank : mt) * kBM;
+                const int brow0 = g * p.a.n + nt * kBN + crank * (kBN / 2);  // a CTA of a pair loads half of B
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     const uint32_t stage = issued % kStages;
-                    if (!sm100::mbar_wait(&empty[stage], ((issued / kStages) & 1) ^ 1)) {
+                    if (!sm100::mbar_wait(&done[stage], ((issued / kStages) & 1) ^ 1)) {
                         fail();
                         ok = false;
                         break;
                     }
-                    uint8_t* sa = smem + stage * Smem::kStageBytes;
-                    sm100::mbar_arrive_expect_tx(&full[stage], Smem::kStageBytes);
-                    sm100::tma_load_2d(sa, &tmap_a, &full[stage], kb * kBK, row0);
-                    sm100::tma_load_2d(sa + Smem::kABytes, &tmap_b, &full[stage], kb * kBK, brow0);
+                    uint8_t* sa = smem + stage * S::kStageBytes;
+                    if constexpr (PAIR) {  // both CTAs' loads complete on the leader's barrier
+                        if (crank == 0) sm100::mbar_arrive_expect_tx(&full[stage], 2 * S::kStageBytes);
+                        const uint32_t bar = sm100::mapa(&full[stage], 0);
+                        sm100::tma_load_2d_pair(sa, &tmap_a, bar, kb * kBK, row0);
+                        sm100::tma_load_2d_pair(sa + S::kABytes, &tmap_b, bar, kb * kBK, brow0);
+                    } else {
+                        sm100::mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
+                        sm100::tma_load_2d(sa, &tmap_a, &full[stage], kb * kBK, row0);
+                        sm100::tma_load_2d(sa + S::kABytes, &tmap_b, &full[stage], kb * kBK, brow0);
+                    }
                     ++issued;
                 }
             }
-            // No load may still be in flight when this CTA's shared memory goes away.
+            // No load may still be in flight when this CTA's shared memory goes away:
+            // each has landed once the MMAs that read its stage are done.
             for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
-                if (!sm100::mbar_wait(&full[i % kStages], (i / kStages) & 1)) fail();
+                if (!sm100::mbar_wait(&done[i % kStages], (i / kStages) & 1)) fail();
             }
-        } else if (warp == 9 && lane == 0) {
-            const uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kBN);
+        } else if (warp == 9 && crank == 0) {
+            // The whole warp walks the blocks and one elected lane issues, so that
+            // descriptors and addresses are warp-uniform.
+            const uint32_t idesc = sm100::idesc_e4m3_f32(PAIR ? 2 * kBM : kBM, kBN);
+            const uint64_t desc0 = sm100::sw128_kmajor_desc(smem);
+            const bool issuer = sm100::elect_one();
             uint32_t it = 0;
+            uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
+            for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
                 for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                    const uint32_t stage = it % kStages;
                     const uint32_t buf = it & 1;
-                    if (!sm100::mbar_wait(&tmem_empty[buf], ((it >> 1) & 1) ^ 1) ||
-                        !sm100::mbar_wait(&full[stage], (it / kStages) & 1)) {
-                        fail();
-                        ok = false;
+                    ok = sm100::mbar_wait(&full[stage], phase) && sm100::mbar_wait(&tmem_empty[buf], ((it >> 1) & 1) ^ 1);
+                    if (!ok) {
+                        if (issuer) fail();
                         break;
                     }
                     sm100::tc_fence_after();
-                    uint8_t* sa = smem + stage * Smem::kStageBytes;
-                    const uint64_t ad = sm100::sw128_kmajor_desc(sa);
-                    const uint64_t bd = sm100::sw128_kmajor_desc(sa + Smem::kABytes);
+                    const uint64_t ad = desc0 + stage * (S::kStageBytes >> 4);
+                    const uint64_t bd = ad + (S::kABytes >> 4);
+                    const uint32_t d = tmem_base + buf * kBN;
+                    if (issuer) {
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 32; ++kk) {  // 32 bytes of K = 2 descriptor units a step
-                        sm100::mma_f8(tmem_base + buf * kBN, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                        for (int kk = 0; kk < kBK / 32; ++kk) {  // 32 bytes of K = 2 descriptor units a step
+                            if constexpr (PAIR) sm100::mma_f8_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                            else sm100::mma_f8(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                        }
+                        if constexpr (PAIR) sm100::mma_commit_both(&done[stage]);
+                        else sm100::mma_commit(&done[stage]);
                     }
-                    sm100::mma_commit(&empty[stage]);
-                    sm100::mma_commit(&tmem_full[buf]);
+                    __syncwarp();
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
             }
             // Nor may an MMA still write the TMEM that is freed below.
-            if (it > 0 && !sm100::mbar_wait(&tmem_full[(it - 1) & 1], ((it - 1) >> 1) & 1)) fail();
+            if (it > 0 && !sm100::mbar_wait(&done[(it - 1) % kStages], ((it - 1) / kStages) & 1)) fail();
         }
     } else {
         sm100::reg_inc<kDrainRegs>();
@@ -230,10 +264,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t it = 0;
         uint32_t n_done = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x, ++n_done) {
+        for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step, ++n_done) {
             int g, mt, nt;
             find_tile(table, groups, n_tiles, tile, g, mt, nt);
-            const int64_t row = static_cast<int64_t>(table.off[g]) + mt * kBM + row_in_tile;
+            const int64_t row = static_cast<int64_t>(table.off[g]) + (PAIR ? 2 * mt + crank : mt) * kBM + row_in_tile;
             const bool valid = row < table.off[g + 1];
             const float* sa = p.a.a_scale + (valid ? row : 0) * p.a.a_scale_stride;
             const int bb = nt * 2;
@@ -252,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     b1_next = __ldg(sb1 + kb + 1);
                 }
                 const uint32_t buf = it & 1;
-                if (!sm100::mbar_wait(&tmem_full[buf], (it >> 1) & 1)) {
+                if (!sm100::mbar_wait(&done[it % kStages], (it / kStages) & 1)) {
                     fail();
                     ok = false;
                     break;
@@ -261,16 +295,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t taddr =
                     tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + static_cast<uint32_t>(half * 64);
                 const uint64_t ss0 = pack2(s0, s0), ss1 = pack2(s1, s1);
+                // Four loads of 32 columns; each but the first runs under the
+                // multiply-adds of the one before.
+                uint32_t v[2][32];
+                sm100::tmem_issue_32cols(taddr, v[0]);
+                sm100::tmem_wait_32cols(v[0]);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    float v[32];
-                    sm100::tmem_ld_32cols(taddr + (c >> 1) * 128 + (c & 1) * 32, v);
+                    if (c < 3) {
+                        sm100::tmem_issue_32cols(taddr + ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 32, v[(c + 1) & 1]);
+                    } else {  // all of the accumulator is in registers: the next MMAs may have it
+                        sm100::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (PAIR) sm100::mbar_arrive_remote(sm100::mapa(&tmem_empty[buf], 0));
+                            else sm100::mbar_arrive(&tmem_empty[buf]);
+                        }
+                    }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], pack2(v[2 * i], v[2 * i + 1]), c < 2 ? ss0 : ss1);
+                    for (int i = 0; i < 16; ++i) {
+                        fma2(acc[c * 16 + i], pack2(v[c & 1][2 * i], v[c & 1][2 * i + 1]), c < 2 ? ss0 : ss1);
+                    }
+                    if (c < 3) sm100::tmem_wait_32cols(v[(c + 1) & 1]);
                 }
-                sm100::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) sm100::mbar_arrive(&tmem_empty[buf]);
             }
             if (!ok) break;
             if constexpr (EPI == kEpiStore) {
@@ -352,8 +399,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     sm100::tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) sm100::cluster_sync();  // neither CTA leaves while the other may touch its barriers
     sm100::tc_fence_after();
-    if (warp == 9) sm100::tmem_dealloc(tmem_base, 2 * kBN);
+    if (warp == 9) {
+        if constexpr (PAIR) sm100::tmem_dealloc_pair(tmem_base, 2 * kBN);
+        else sm100::tmem_dealloc(tmem_base, 2 * kBN);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -427,12 +478,37 @@ __global__ void __launch_bounds__(256) quant_fp8_blocks_kernel(const __nv_bfloat
 
 __device__ uint32_t g_error;
 
-template <int EPI>
-void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int grid, cudaStream_t stream) {
+bool use_pair(const Fp8GemmArgs& a, int64_t n_tiles) {
+    static const int force = getenv("KIWI_PAIR") ? atoi(getenv("KIWI_PAIR")) : -1;
+    if (force >= 0) return force;
+    return false;
+}
+
+template <int EPI, bool PAIR>
+void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int64_t most_tiles, cudaStream_t stream) {
     static std::atomic<uint64_t> attr{0};
-    raise_smem_limit(reinterpret_cast<const void*>(fp8_gemm_kernel<EPI>), Smem::kBytes, attr);
-    fp8_gemm_kernel<EPI><<<grid, kThreads, Smem::kBytes, stream>>>(ta, tb, p);
-    KIWI_CUDA_CHECK(cudaGetLastError());
+    constexpr int smem = Smem<PAIR>::kBytes;
+    raise_smem_limit(reinterpret_cast<const void*>(fp8_gemm_kernel<EPI, PAIR>), smem, attr);
+    const int64_t workers = PAIR ? num_sms() / 2 : num_sms();
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim = {2, 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(most_tiles < workers ? most_tiles : workers) * (PAIR ? 2 : 1));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    KIWI_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<EPI, PAIR>, ta, tb, p));
+}
+
+template <bool PAIR>
+void launch_epi(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int64_t most_tiles,
+                cudaStream_t stream) {
+    if (!p.a.swiglu) launch<kEpiStore, PAIR>(ta, tb, p, most_tiles, stream);
+    else if (!p.a.codes) launch<kEpiSwiGLU, PAIR>(ta, tb, p, most_tiles, stream);
+    else launch<kEpiSwiGLUQuant, PAIR>(ta, tb, p, most_tiles, stream);
 }
 
 }  // namespace
@@ -469,16 +545,15 @@ void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream) {
     p.nb = (args.n + 127) / 128;
     p.error = gemm_error_word();
     const CUtensorMap ta = make_tmap_2d(args.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, args.rows, args.k, args.lda, kBM, kBK);
-    const CUtensorMap tb = make_tmap_2d(args.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1,
-                                        static_cast<uint64_t>(args.num_groups) * args.n, args.k, args.ldb, kBN, kBK);
-    // At most this many tiles, however the rows fall into groups.
     const int64_t n_tiles = (args.n + kBN - 1) / kBN;
-    const int64_t most = ((args.rows + kBM - 1) / kBM + (args.counts ? args.num_groups : 0)) * n_tiles;
-    const int sms = num_sms();
-    const int grid = static_cast<int>(most < sms ? most : sms);
-    if (!args.swiglu) launch<kEpiStore>(ta, tb, p, grid, stream);
-    else if (!args.codes) launch<kEpiSwiGLU>(ta, tb, p, grid, stream);
-    else launch<kEpiSwiGLUQuant>(ta, tb, p, grid, stream);
+    // At most this many tiles of bm rows, however the rows fall into groups.
+    auto most = [&](int64_t bm) { return ((args.rows + bm - 1) / bm + (args.counts ? args.num_groups : 0)) * n_tiles; };
+    const bool pair = use_pair(args, n_tiles);
+    const CUtensorMap tb =
+        make_tmap_2d(args.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, static_cast<uint64_t>(args.num_groups) * args.n, args.k,
+                     args.ldb, pair ? kBN / 2 : kBN, kBK);
+    if (pair) launch_epi<true>(ta, tb, p, most(2 * kBM), stream);
+    else launch_epi<false>(ta, tb, p, most(kBM), stream);
 }
 
 void quant_fp8_blocks(const __nv_bfloat16* w, int64_t ld, int64_t rows, int64_t cols, uint8_t* codes, float* scales,
