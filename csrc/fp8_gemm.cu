@@ -21,7 +21,8 @@
 //                h = warp / 4, so that with SwiGLU a thread owns matching gate
 //                and up columns; 128 fp32 sums in registers
 //   warp 8       TMA producer: 128 x 128-byte A tile + 256 x 128-byte B tile
-//   warp 9       TMEM owner and MMA issuer (warps 10 and 11 only fill its warpgroup)
+//   warp 9       TMEM owner and MMA issuer
+//   warps 10..11 scales: sa * sb of every row, a block ahead, to shared memory
 // Every wait is bounded; one that runs out sets the error word, and the CTA
 // drains its loads, frees its TMEM and leaves.
 #include <cuda.h>
@@ -47,11 +48,12 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kBN = 256;
 constexpr int kBK = 128;      // bytes = e4m3 elements = one scale block
-constexpr int kThreads = 384;  // two drain warpgroups; one with the producer, the MMA issuer and two idle warps
+constexpr int kThreads = 384;  // two drain warpgroups; one with the producer, the MMA issuer and the scale warps
 constexpr int kDrainThreads = 256;
+constexpr int kScaleWarps = 2;
 // 128 sums and a 32-column TMEM load do not fit the 168 registers that 384
 // threads share evenly; the third warpgroup gives some of its own away.
-constexpr int kDrainRegs = 232, kIssueRegs = 40;
+constexpr int kDrainRegs = 200, kIssueRegs = 104;
 static_assert(2 * kDrainRegs + kIssueRegs <= 3 * 168, "more registers than the CTA is launched with");
 
 enum Epi : int { kEpiStore = 0, kEpiSwiGLU = 1, kEpiSwiGLUQuant = 2 };
@@ -64,7 +66,8 @@ struct Smem {
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kTableOffset = kStages * kStageBytes;
     static constexpr int kAmaxOffset = kTableOffset + static_cast<int>(round_up(sizeof(GroupTable), 16));
-    static constexpr int kBarOffset = kAmaxOffset + 2 * 2 * kBM * 4;
+    static constexpr int kScaleOffset = kAmaxOffset + 2 * 2 * kBM * 4;
+    static constexpr int kBarOffset = kScaleOffset + 2 * kBM * 8;
     static constexpr int kBytes = kBarOffset + 256 + 1024;  // barriers, TMEM slot, alignment slack
 };
 static_assert(Smem<false>::kBytes <= 227 * 1024 && Smem<true>::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
@@ -129,10 +132,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     GroupTable& table = *reinterpret_cast<GroupTable*>(smem + S::kTableOffset);
     float* s_amax = reinterpret_cast<float*>(smem + S::kAmaxOffset);  // [tile parity][column half][row]
+    float2* s_scale = reinterpret_cast<float2*>(smem + S::kScaleOffset);  // [block parity][row]: for each column part
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBarOffset);
-    uint64_t* done = full + kStages;  // a stage's MMAs: its operands may be overwritten, its partial sums drained
-    uint64_t* tmem_empty = done + kStages;
-    uint64_t* amax_bar = tmem_empty + 2;
+    // done: a block's MMAs have run and its scales are in shared memory.  Its
+    // operands may be overwritten, its partial sums drained.
+    uint64_t* done = full + kStages;
+    uint64_t* tmem_empty = done + kStages;                          // in a pair, the leader's counts both CTAs
+    uint64_t* drained = PAIR ? tmem_empty + 2 : tmem_empty;         // this CTA's drain of a block
+    uint64_t* amax_bar = tmem_empty + 4;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(amax_bar + 1);
     __shared__ int s_abort;
 
@@ -149,10 +156,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_abort = 0;
         for (int s = 0; s < kStages; ++s) {
             sm100::mbar_init(&full[s], 1);
-            sm100::mbar_init(&done[s], 1);
+            sm100::mbar_init(&done[s], 1 + kScaleWarps);
         }
         for (int i = 0; i < 2; ++i) {
             sm100::mbar_init(&tmem_empty[i], (PAIR ? 2 : 1) * kDrainThreads / 32);
+            if (PAIR) sm100::mbar_init(&drained[i], kDrainThreads / 32);
         }
         sm100::mbar_init(amax_bar, kDrainThreads);
         sm100::fence_mbar_init();
@@ -253,7 +261,45 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             // Nor may an MMA still write the TMEM that is freed below.
-            if (it > 0 && !sm100::mbar_wait(&done[(it - 1) % kStages], ((it - 1) / kStages) & 1)) fail();
+            if (it > 0 && !sm100::mbar_wait(&done[(it - 1) % kStages], ((it - 1) / kStages) & 1) && issuer) fail();
+        } else if (warp >= 10) {
+            // Scale warps: each lane multiplies two rows' scales with those of the
+            // tile's two column parts, a block ahead of the drain.
+            uint32_t it = 0;
+            uint32_t stage = 0;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
+                int g, mt, nt;
+                find_tile(table, groups, n_tiles, tile, g, mt, nt);
+                const int r = (warp - 10) * 64 + lane;
+                const int64_t row = static_cast<int64_t>(table.off[g]) + (PAIR ? 2 * mt + crank : mt) * kBM + r;
+                const int64_t last = table.off[g + 1] - 1;  // rows past the group's are not stored: any scale will do
+                const float* sa0 = p.a.a_scale + (row < last ? row : last) * p.a.a_scale_stride;
+                const float* sa1 = p.a.a_scale + (row + 32 < last ? row + 32 : last) * p.a.a_scale_stride;
+                const float* sb0 = p.a.b_scale + (static_cast<int64_t>(g) * p.nb + 2 * nt) * k_blocks;
+                const float* sb1 = 2 * nt + 1 < p.nb ? sb0 + k_blocks : sb0;
+                float a0 = __ldg(sa0), a1 = __ldg(sa1), b0 = __ldg(sb0), b1 = __ldg(sb1);
+                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                    const float2 v0 = make_float2(a0 * b0, a0 * b1), v1 = make_float2(a1 * b0, a1 * b1);
+                    if (kb + 1 < k_blocks) {
+                        a0 = __ldg(sa0 + kb + 1);
+                        a1 = __ldg(sa1 + kb + 1);
+                        b0 = __ldg(sb0 + kb + 1);
+                        b1 = __ldg(sb1 + kb + 1);
+                    }
+                    const uint32_t buf = it & 1;
+                    if (!sm100::mbar_wait(&drained[buf], ((it >> 1) & 1) ^ 1)) {
+                        if (lane == 0) fail();
+                        ok = false;
+                        break;
+                    }
+                    s_scale[buf * kBM + r] = v0;
+                    s_scale[buf * kBM + r + 32] = v1;
+                    __syncwarp();
+                    if (lane == 0) sm100::mbar_arrive(&done[stage]);
+                    if (++stage == kStages) stage = 0;
+                }
+            }
         }
     } else {
         sm100::reg_inc<kDrainRegs>();
@@ -262,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row_in_tile = q * 32 + lane;
         const bool vec = p.a.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.a.c) % 16 == 0;
         uint32_t it = 0;
+        uint32_t stage = 0, phase = 0;
         uint32_t n_done = 0;
         bool ok = true;
         for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step, ++n_done) {
@@ -269,24 +316,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             find_tile(table, groups, n_tiles, tile, g, mt, nt);
             const int64_t row = static_cast<int64_t>(table.off[g]) + (PAIR ? 2 * mt + crank : mt) * kBM + row_in_tile;
             const bool valid = row < table.off[g + 1];
-            const float* sa = p.a.a_scale + (valid ? row : 0) * p.a.a_scale_stride;
-            const int bb = nt * 2;
-            const float* sb0 = p.a.b_scale + (static_cast<int64_t>(g) * p.nb + bb) * k_blocks;
-            const float* sb1 = bb + 1 < p.nb ? sb0 + k_blocks : sb0;
-            float a_next = __ldg(sa), b0_next = __ldg(sb0), b1_next = __ldg(sb1);
             uint64_t acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
 #pragma unroll 1
             for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                const float s0 = a_next * b0_next, s1 = a_next * b1_next;
-                if (kb + 1 < k_blocks) {  // the next block's scales travel while this one's MMAs run
-                    a_next = __ldg(sa + kb + 1);
-                    b0_next = __ldg(sb0 + kb + 1);
-                    b1_next = __ldg(sb1 + kb + 1);
-                }
                 const uint32_t buf = it & 1;
-                if (!sm100::mbar_wait(&done[it % kStages], (it / kStages) & 1)) {
+                if (!sm100::mbar_wait(&done[stage], phase)) {
                     fail();
                     ok = false;
                     break;
@@ -294,7 +330,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sm100::tc_fence_after();
                 const uint32_t taddr =
                     tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + static_cast<uint32_t>(half * 64);
-                const uint64_t ss0 = pack2(s0, s0), ss1 = pack2(s1, s1);
+                const float2 sc = s_scale[buf * kBM + row_in_tile];
+                const uint64_t ss0 = pack2(sc.x, sc.x), ss1 = pack2(sc.y, sc.y);
                 // Four loads of 32 columns; each but the first runs under the
                 // multiply-adds of the one before.
                 uint32_t v[2][32];
@@ -309,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         __syncwarp();
                         if (lane == 0) {
                             if constexpr (PAIR) sm100::mbar_arrive_remote(sm100::mapa(&tmem_empty[buf], 0));
-                            else sm100::mbar_arrive(&tmem_empty[buf]);
+                            sm100::mbar_arrive(&drained[buf]);
                         }
                     }
 #pragma unroll
@@ -317,6 +354,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         fma2(acc[c * 16 + i], pack2(v[c & 1][2 * i], v[c & 1][2 * i + 1]), c < 2 ? ss0 : ss1);
                     }
                     if (c < 3) sm100::tmem_wait_32cols(v[(c + 1) & 1]);
+                }
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
                 }
             }
             if (!ok) break;
