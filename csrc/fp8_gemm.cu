@@ -38,6 +38,7 @@
 #include "kiwi/gemm/fp8_gemm.hpp"
 #include "kiwi/gemm/group_table.cuh"
 #include "kiwi/gemm/grouped_gemm.hpp"
+#include "kiwi/gemm/row_store.cuh"
 #include "kiwi/gemm/tensor_map.hpp"
 #include "kiwi/sm100.cuh"
 
@@ -67,7 +68,8 @@ struct Smem {
     static constexpr int kTableOffset = kStages * kStageBytes;
     static constexpr int kAmaxOffset = kTableOffset + static_cast<int>(round_up(sizeof(GroupTable), 16));
     static constexpr int kScaleOffset = kAmaxOffset + 2 * 2 * kBM * 4;
-    static constexpr int kBarOffset = kScaleOffset + 2 * kBM * 8;
+    static constexpr int kStgOffset = kScaleOffset + 2 * kBM * 8;
+    static constexpr int kBarOffset = kStgOffset + kDrainThreads / 32 * kRowStoreBytes;
     static constexpr int kBytes = kBarOffset + 256 + 1024;  // barriers, TMEM slot, alignment slack
 };
 static_assert(Smem<false>::kBytes <= 227 * 1024 && Smem<true>::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
@@ -104,21 +106,34 @@ __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) {
 
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
 
-/// 64 consecutive columns of one row as bf16, `cols` of them inside the matrix.
-__device__ __forceinline__ void store_row64(__nv_bfloat16* dst, const float (&v)[64], int cols, bool vec) {
+/// The warp's rows' 64 columns at `col` as bf16: row r0 + lane from v, of which
+/// rows before `rows` and columns before `cols` are in the matrix.
+__device__ __forceinline__ void store_rows(__nv_bfloat16* c, int64_t ldc, int64_t r0, int rows, int col, int cols,
+                                           const float (&v)[64], uint8_t* stg, bool vec) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float f[8];
+    for (int h = 0; h < 2; ++h) {  // 32 columns = 64 bytes a row
+        uint4 w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = v[8 * j + i];
-        if (vec && 8 * j + 8 <= cols) {
-            *reinterpret_cast<uint4*>(dst + 8 * j) = ep::f32x8_to_bf16(f);
-        } else {
+        for (int j = 0; j < 4; ++j) {
+            float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (8 * j + i < cols) dst[8 * j + i] = __float2bfloat16_rn(f[i]);
-            }
+            for (int i = 0; i < 8; ++i) f[i] = v[32 * h + 8 * j + i];
+            w[j] = ep::f32x8_to_bf16(f);
         }
+        emit_rows64(stg, w, [&](int row, int piece, const uint4& x) {
+            const int at = col + 32 * h + 8 * piece;
+            if (row >= rows || at >= cols) return;
+            __nv_bfloat16* dst = c + (r0 + row) * ldc + at;
+            if (vec && at + 8 <= cols) {
+                *reinterpret_cast<uint4*>(dst) = x;
+            } else {
+                const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (at + i < cols) dst[i] = e[i];
+                }
+            }
+        });
     }
 }
 
@@ -306,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int q = warp & 3;
         const int half = warp >> 2;
         const int row_in_tile = q * 32 + lane;
+        uint8_t* stg = smem + S::kStgOffset + warp * kRowStoreBytes;
         const bool vec = p.a.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.a.c) % 16 == 0;
         uint32_t it = 0;
         uint32_t stage = 0, phase = 0;
@@ -316,6 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             find_tile(table, groups, n_tiles, tile, g, mt, nt);
             const int64_t row = static_cast<int64_t>(table.off[g]) + (PAIR ? 2 * mt + crank : mt) * kBM + row_in_tile;
             const bool valid = row < table.off[g + 1];
+            const int64_t r0 = row - lane;  // the warp's first row, and how many of its rows are the group's
+            const int r_end = static_cast<int>(table.off[g + 1] - r0 < 32 ? table.off[g + 1] - r0 : 32);
             uint64_t acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
@@ -373,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         v[2 * i + 1] = f.y * scale;
                     }
                     const int col = nt * kBN + part * 128 + half * 64;
-                    if (valid && col < p.a.n) store_row64(p.a.c + row * p.a.ldc + col, v, p.a.n - col, vec);
+                    store_rows(p.a.c, p.a.ldc, r0, r_end, col, p.a.n, v, stg, vec);
                 }
             } else {
                 float h[64];
@@ -389,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float scale = valid && p.a.row_scale ? __ldg(p.a.row_scale + row) : 1.0f;
 #pragma unroll
                     for (int i = 0; i < 64; ++i) h[i] *= scale;
-                    if (valid) store_row64(p.a.c + row * p.a.ldc + col, h, 64, vec);
+                    store_rows(p.a.c, p.a.ldc, r0, r_end, col, p.a.n / 2, h, stg, vec);
                 } else {
                     // The tile's 128 hidden columns are one scale block; its other 64
                     // columns are in the thread of the same row in the other four warps.
@@ -406,21 +424,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                     amax = fmaxf(amax, slot[(half ^ 1) * kBM + row_in_tile]);
                     const float scale = amax > 0.f ? amax / ep::kFp8Max : 1.0f;
                     const float inv = amax > 0.f ? ep::kFp8Max / amax : 0.f;
-                    if (valid) {
-                        uint32_t w[16];
+                    uint4 w[4];
+                    uint32_t* wi = reinterpret_cast<uint32_t*>(w);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint32_t lo = __nv_cvt_float2_to_fp8x2(
-                                make_float2(h[4 * i] * inv, h[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                            const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-                                make_float2(h[4 * i + 2] * inv, h[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-                            w[i] = lo | (hi << 16);
-                        }
-                        uint4* dst = reinterpret_cast<uint4*>(p.a.codes + row * (p.a.n / 2) + col);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                        if (half == 0) p.a.scales[row * (p.a.n / kBN) + nt] = scale;
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(h[4 * i] * inv, h[4 * i + 1] * inv),
+                                                                     __NV_SATFINITE, __NV_E4M3);
+                        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(h[4 * i + 2] * inv, h[4 * i + 3] * inv),
+                                                                     __NV_SATFINITE, __NV_E4M3);
+                        wi[i] = lo | (hi << 16);
                     }
+                    emit_rows64(stg, w, [&](int r, int piece, const uint4& x) {
+                        if (r < r_end) *reinterpret_cast<uint4*>(p.a.codes + (r0 + r) * (p.a.n / 2) + col + 16 * piece) = x;
+                    });
+                    if (valid && half == 0) p.a.scales[row * (p.a.n / kBN) + nt] = scale;
                 }
             }
         }
