@@ -30,11 +30,13 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
-#include <cstdlib>
+#include <cmath>
 #include <mutex>
 
 #include "kiwi/ep/quant.cuh"
+#include "kiwi/gemm/fp8_detail.cuh"
 #include "kiwi/gemm/fp8_gemm.hpp"
 #include "kiwi/gemm/group_table.cuh"
 #include "kiwi/gemm/grouped_gemm.hpp"
@@ -46,24 +48,21 @@ namespace kiwi::gemm {
 
 namespace {
 
+using namespace fp8;
+
 constexpr int kBM = 128;
-constexpr int kBN = 256;
-constexpr int kBK = 128;      // bytes = e4m3 elements = one scale block
 constexpr int kThreads = 384;  // two drain warpgroups; one with the producer, the MMA issuer and the scale warps
 constexpr int kDrainThreads = 256;
 constexpr int kScaleWarps = 2;
 // 128 sums and a 32-column TMEM load do not fit the 168 registers that 384
 // threads share evenly; the third warpgroup gives some of its own away.
-constexpr int kDrainRegs = 200, kIssueRegs = 104;
+constexpr int kDrainRegs = 208, kIssueRegs = 88;
 static_assert(2 * kDrainRegs + kIssueRegs <= 3 * 168, "more registers than the CTA is launched with");
 
-enum Epi : int { kEpiStore = 0, kEpiSwiGLU = 1, kEpiSwiGLUQuant = 2 };
-
-template <bool PAIR>
 struct Smem {
-    static constexpr int kStages = PAIR ? 6 : 4;
+    static constexpr int kStages = 4;
     static constexpr int kABytes = kBM * kBK;
-    static constexpr int kBBytes = (PAIR ? kBN / 2 : kBN) * kBK;
+    static constexpr int kBBytes = kBN * kBK;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kTableOffset = kStages * kStageBytes;
     static constexpr int kAmaxOffset = kTableOffset + static_cast<int>(round_up(sizeof(GroupTable), 16));
@@ -72,39 +71,7 @@ struct Smem {
     static constexpr int kBarOffset = kStgOffset + kDrainThreads / 32 * kRowStoreBytes;
     static constexpr int kBytes = kBarOffset + 256 + 1024;  // barriers, TMEM slot, alignment slack
 };
-static_assert(Smem<false>::kBytes <= 227 * 1024 && Smem<true>::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
-
-struct Params {
-    Fp8GemmArgs a;
-    int k_blocks;
-    int nb;  // scale blocks of B per group along n
-    uint32_t* error;
-};
-
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-}
-
-/// acc += v * s on two fp32 lanes (one instruction).
-__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
-}
-
-__device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
+static_assert(Smem::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
 
 /// The warp's rows' 64 columns at `col` as bf16: row r0 + lane from v, of which
 /// rows before `rows` and columns before `cols` are in the matrix.
@@ -120,28 +87,18 @@ __device__ __forceinline__ void store_rows(__nv_bfloat16* c, int64_t ldc, int64_
             for (int i = 0; i < 8; ++i) f[i] = v[32 * h + 8 * j + i];
             w[j] = ep::f32x8_to_bf16(f);
         }
-        emit_rows64(stg, w, [&](int row, int piece, const uint4& x) {
-            const int at = col + 32 * h + 8 * piece;
-            if (row >= rows || at >= cols) return;
-            __nv_bfloat16* dst = c + (r0 + row) * ldc + at;
-            if (vec && at + 8 <= cols) {
-                *reinterpret_cast<uint4*>(dst) = x;
-            } else {
-                const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (at + i < cols) dst[i] = e[i];
-                }
-            }
-        });
+        const int at = col + 32 * h;
+        if (rows > 0 && at < cols) {
+            store_rows64(stg, w, reinterpret_cast<uint8_t*>(c + r0 * ldc + at), ldc * 2, rows, (cols - at) * 2, vec);
+        }
     }
 }
 
-template <int EPI, bool PAIR>
+template <int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const __grid_constant__ Params p) {
-    using S = Smem<PAIR>;
+    using S = Smem;
     constexpr int kStages = S::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -152,9 +109,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // done: a block's MMAs have run and its scales are in shared memory.  Its
     // operands may be overwritten, its partial sums drained.
     uint64_t* done = full + kStages;
-    uint64_t* tmem_empty = done + kStages;                          // in a pair, the leader's counts both CTAs
-    uint64_t* drained = PAIR ? tmem_empty + 2 : tmem_empty;         // this CTA's drain of a block
-    uint64_t* amax_bar = tmem_empty + 4;
+    uint64_t* drained = done + kStages;  // [block parity] an accumulator and its scales have been read
+    uint64_t* amax_bar = drained + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(amax_bar + 1);
     __shared__ int s_abort;
 
@@ -163,9 +119,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int groups = p.a.num_groups;
     const int n_tiles = (p.a.n + kBN - 1) / kBN;
     const int k_blocks = p.k_blocks;
-    const int crank = PAIR ? static_cast<int>(sm100::cluster_ctarank()) : 0;
-    const int first_tile = PAIR ? blockIdx.x / 2 : blockIdx.x;
-    const int tile_step = PAIR ? gridDim.x / 2 : gridDim.x;
 
     if (threadIdx.x == 0) {
         s_abort = 0;
@@ -174,8 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             sm100::mbar_init(&done[s], 1 + kScaleWarps);
         }
         for (int i = 0; i < 2; ++i) {
-            sm100::mbar_init(&tmem_empty[i], (PAIR ? 2 : 1) * kDrainThreads / 32);
-            if (PAIR) sm100::mbar_init(&drained[i], kDrainThreads / 32);
+            sm100::mbar_init(&drained[i], kDrainThreads / 32);
         }
         sm100::mbar_init(amax_bar, kDrainThreads);
         sm100::fence_mbar_init();
@@ -185,13 +137,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::tma_prefetch_desc(&tmap_b);
     }
     if (warp == 9) {
-        if constexpr (PAIR) sm100::tmem_alloc_pair(tmem_slot, 2 * kBN);
-        else sm100::tmem_alloc(tmem_slot, 2 * kBN);
+        sm100::tmem_alloc(tmem_slot, 2 * kBN);
     }
-    build_group_table(table, p.a.counts, groups, p.a.rows, PAIR ? 2 * kBM : kBM, n_tiles, p.error);
+    build_group_table(table, p.a.counts, groups, p.a.rows, kBM, n_tiles, p.error);
     sm100::tc_fence_before();
     __syncthreads();
-    if constexpr (PAIR) sm100::cluster_sync();  // both CTAs' barriers exist before any arrival from the other
     sm100::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = table.tiles[groups];
@@ -207,11 +157,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 8 && lane == 0) {
             uint32_t issued = 0;
             bool ok = true;
-            for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
+            for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
                 int g, mt, nt;
                 find_tile(table, groups, n_tiles, tile, g, mt, nt);
-                const int row0 = table.off[g] + (PAIR ? 2 * mt + crank : mt) * kBM;
-                const int brow0 = g * p.a.n + nt * kBN + crank * (kBN / 2);  // a CTA of a pair loads half of B
+                const int row0 = table.off[g] + mt * kBM;
+                const int brow0 = g * p.a.n + nt * kBN;
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     const uint32_t stage = issued % kStages;
                     if (!sm100::mbar_wait(&done[stage], ((issued / kStages) & 1) ^ 1)) {
@@ -220,16 +170,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         break;
                     }
                     uint8_t* sa = smem + stage * S::kStageBytes;
-                    if constexpr (PAIR) {  // both CTAs' loads complete on the leader's barrier
-                        if (crank == 0) sm100::mbar_arrive_expect_tx(&full[stage], 2 * S::kStageBytes);
-                        const uint32_t bar = sm100::mapa(&full[stage], 0);
-                        sm100::tma_load_2d_pair(sa, &tmap_a, bar, kb * kBK, row0);
-                        sm100::tma_load_2d_pair(sa + S::kABytes, &tmap_b, bar, kb * kBK, brow0);
-                    } else {
-                        sm100::mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
-                        sm100::tma_load_2d(sa, &tmap_a, &full[stage], kb * kBK, row0);
-                        sm100::tma_load_2d(sa + S::kABytes, &tmap_b, &full[stage], kb * kBK, brow0);
-                    }
+                    sm100::mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
+                    sm100::tma_load_2d(sa, &tmap_a, &full[stage], kb * kBK, row0);
+                    sm100::tma_load_2d(sa + S::kABytes, &tmap_b, &full[stage], kb * kBK, brow0);
                     ++issued;
                 }
             }
@@ -238,19 +181,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
                 if (!sm100::mbar_wait(&done[i % kStages], (i / kStages) & 1)) fail();
             }
-        } else if (warp == 9 && crank == 0) {
+        } else if (warp == 9) {
             // The whole warp walks the blocks and one elected lane issues, so that
             // descriptors and addresses are warp-uniform.
-            const uint32_t idesc = sm100::idesc_e4m3_f32(PAIR ? 2 * kBM : kBM, kBN);
+            const uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kBN);
             const uint64_t desc0 = sm100::sw128_kmajor_desc(smem);
             const bool issuer = sm100::elect_one();
             uint32_t it = 0;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
+            for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
                 for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                     const uint32_t buf = it & 1;
-                    ok = sm100::mbar_wait(&full[stage], phase) && sm100::mbar_wait(&tmem_empty[buf], ((it >> 1) & 1) ^ 1);
+                    ok = sm100::mbar_wait(&full[stage], phase) && sm100::mbar_wait(&drained[buf], ((it >> 1) & 1) ^ 1);
                     if (!ok) {
                         if (issuer) fail();
                         break;
@@ -262,11 +205,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (issuer) {
 #pragma unroll
                         for (int kk = 0; kk < kBK / 32; ++kk) {  // 32 bytes of K = 2 descriptor units a step
-                            if constexpr (PAIR) sm100::mma_f8_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0 ? 1u : 0u);
-                            else sm100::mma_f8(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                            sm100::mma_f8(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0 ? 1u : 0u);
                         }
-                        if constexpr (PAIR) sm100::mma_commit_both(&done[stage]);
-                        else sm100::mma_commit(&done[stage]);
+                        sm100::mma_commit(&done[stage]);
                     }
                     __syncwarp();
                     if (++stage == kStages) {
@@ -283,11 +224,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t it = 0;
             uint32_t stage = 0;
             bool ok = true;
-            for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
+            for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
                 int g, mt, nt;
                 find_tile(table, groups, n_tiles, tile, g, mt, nt);
                 const int r = (warp - 10) * 64 + lane;
-                const int64_t row = static_cast<int64_t>(table.off[g]) + (PAIR ? 2 * mt + crank : mt) * kBM + r;
+                const int64_t row = static_cast<int64_t>(table.off[g]) + mt * kBM + r;
                 const int64_t last = table.off[g + 1] - 1;  // rows past the group's are not stored: any scale will do
                 const float* sa0 = p.a.a_scale + (row < last ? row : last) * p.a.a_scale_stride;
                 const float* sa1 = p.a.a_scale + (row + 32 < last ? row + 32 : last) * p.a.a_scale_stride;
@@ -327,10 +268,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t stage = 0, phase = 0;
         uint32_t n_done = 0;
         bool ok = true;
-        for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step, ++n_done) {
+        for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x, ++n_done) {
             int g, mt, nt;
             find_tile(table, groups, n_tiles, tile, g, mt, nt);
-            const int64_t row = static_cast<int64_t>(table.off[g]) + (PAIR ? 2 * mt + crank : mt) * kBM + row_in_tile;
+            const int64_t row = static_cast<int64_t>(table.off[g]) + mt * kBM + row_in_tile;
             const bool valid = row < table.off[g + 1];
             const int64_t r0 = row - lane;  // the warp's first row, and how many of its rows are the group's
             const int r_end = static_cast<int>(table.off[g + 1] - r0 < 32 ? table.off[g + 1] - r0 : 32);
@@ -363,7 +304,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         sm100::tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
-                            if constexpr (PAIR) sm100::mbar_arrive_remote(sm100::mapa(&tmem_empty[buf], 0));
                             sm100::mbar_arrive(&drained[buf]);
                         }
                     }
@@ -434,9 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                                      __NV_SATFINITE, __NV_E4M3);
                         wi[i] = lo | (hi << 16);
                     }
-                    emit_rows64(stg, w, [&](int r, int piece, const uint4& x) {
-                        if (r < r_end) *reinterpret_cast<uint4*>(p.a.codes + (r0 + r) * (p.a.n / 2) + col + 16 * piece) = x;
-                    });
+                    if (r_end > 0) store_rows64(stg, w, p.a.codes + r0 * (p.a.n / 2) + col, p.a.n / 2, r_end, 64, true);
                     if (valid && half == 0) p.a.scales[row * (p.a.n / kBN) + nt] = scale;
                 }
             }
@@ -444,24 +382,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.a.zero_tail) {
             const int cols = EPI == kEpiStore ? p.a.n : p.a.n / 2;
             for (int64_t r = table.off[groups] + static_cast<int64_t>(blockIdx.x); r < p.a.rows; r += gridDim.x) {
-                if constexpr (EPI == kEpiSwiGLUQuant) {
-                    for (int c = threadIdx.x * 16; c < cols; c += kDrainThreads * 16) {
-                        *reinterpret_cast<uint4*>(p.a.codes + r * cols + c) = make_uint4(0, 0, 0, 0);
-                    }
-                    for (int c = threadIdx.x; c < cols / 128; c += kDrainThreads) p.a.scales[r * (cols / 128) + c] = 1.0f;
-                } else {
-                    for (int c = threadIdx.x; c < cols; c += kDrainThreads) p.a.c[r * p.a.ldc + c] = __float2bfloat16_rn(0.f);
-                }
+                zero_row<EPI>(p.a, r, cols, threadIdx.x, kDrainThreads);
             }
         }
     }
     sm100::tc_fence_before();
     __syncthreads();
-    if constexpr (PAIR) sm100::cluster_sync();  // neither CTA leaves while the other may touch its barriers
     sm100::tc_fence_after();
     if (warp == 9) {
-        if constexpr (PAIR) sm100::tmem_dealloc_pair(tmem_base, 2 * kBN);
-        else sm100::tmem_dealloc(tmem_base, 2 * kBN);
+        sm100::tmem_dealloc(tmem_base, 2 * kBN);
     }
 }
 
@@ -536,37 +465,64 @@ __global__ void __launch_bounds__(256) quant_fp8_blocks_kernel(const __nv_bfloat
 
 __device__ uint32_t g_error;
 
-bool use_pair(const Fp8GemmArgs& a, int64_t n_tiles) {
-    static const int force = getenv("KIWI_PAIR") ? atoi(getenv("KIWI_PAIR")) : -1;
-    if (force >= 0) return force;
-    return false;
-}
-
-template <int EPI, bool PAIR>
-void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int64_t most_tiles, cudaStream_t stream) {
+template <int EPI>
+void launch(const Params& p, cudaStream_t stream) {
     static std::atomic<uint64_t> attr{0};
-    constexpr int smem = Smem<PAIR>::kBytes;
-    raise_smem_limit(reinterpret_cast<const void*>(fp8_gemm_kernel<EPI, PAIR>), smem, attr);
-    const int64_t workers = PAIR ? num_sms() / 2 : num_sms();
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim = {2, 1, 1};
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(most_tiles < workers ? most_tiles : workers) * (PAIR ? 2 : 1));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = &cluster;
-    cfg.numAttrs = PAIR ? 1 : 0;
-    KIWI_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<EPI, PAIR>, ta, tb, p));
+    raise_smem_limit(reinterpret_cast<const void*>(fp8_gemm_kernel<EPI>), Smem::kBytes, attr);
+    const Fp8GemmArgs& a = p.a;
+    const CUtensorMap ta = make_tmap_2d(a.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.rows, a.k, a.lda, kBM, kBK);
+    const CUtensorMap tb = make_tmap_2d(a.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1,
+                                        static_cast<uint64_t>(a.num_groups) * a.n, a.k, a.ldb, kBN, kBK);
+    // At most this many tiles, however the rows fall into groups.
+    const int64_t most = ((a.rows + kBM - 1) / kBM + (a.counts ? a.num_groups : 0)) * ((a.n + kBN - 1) / kBN);
+    const int sms = num_sms();
+    fp8_gemm_kernel<EPI><<<static_cast<unsigned>(most < sms ? most : sms), kThreads, Smem::kBytes, stream>>>(ta, tb, p);
+    KIWI_CUDA_CHECK(cudaGetLastError());
 }
 
-template <bool PAIR>
-void launch_epi(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, int64_t most_tiles,
-                cudaStream_t stream) {
-    if (!p.a.swiglu) launch<kEpiStore, PAIR>(ta, tb, p, most_tiles, stream);
-    else if (!p.a.codes) launch<kEpiSwiGLU, PAIR>(ta, tb, p, most_tiles, stream);
-    else launch<kEpiSwiGLUQuant, PAIR>(ta, tb, p, most_tiles, stream);
+struct Choice {
+    int row_chunk;  // 0: this file's kernel, else the few-rows kernel with 16 or 32 rows a tile
+    int split;      // and its CTAs a tile
+};
+
+/// The kernel for a call, by a model of its time in microseconds that was fitted
+/// to a sweep of 1 to 2000 rows (dense N x K 512 x 1024 to 7168 x 2048 and 4096 x
+/// 7168; 16 and 32 experts).  A CTA needs 0.42 us a block of K here, and 0.28 or
+/// 0.32 us with 16 or 32 rows a tile, plus 2.5 or 1.2 us a tile for its start
+/// and epilogue.  Where a tile's K is split, the exchange of its sums costs
+/// another 1.3 us, and several times that on a cluster's second tile, so a split
+/// is only for tiles that the GPU runs all at once; clusters of 4 leave some SMs
+/// of a GPC unused, and how rows fall into experts is not known here (every
+/// expert is taken to end with half a tile), hence the margins.  (Splits of 8
+/// lost to splits of 4.)  No kernel is faster than the weights can be read, at
+/// 6.4 TB/s.  Measured, this file's kernel against few rows: 1 row, 4096 x 7168:
+/// 28.7 / 10.1 us; 64 rows: 29.2 / 13.4; 200: 29.9 / 24.4; 400: 30.6 / 44.1; 32
+/// experts of 32 rows, 4096 x 7168: 171 / 154; of 64 rows: 176 / 200.
+Choice choose(const Fp8GemmArgs& a, int k_blocks) {
+    const double sms = num_sms(), n_tiles = (a.n + kBN - 1) / kBN;
+    const double used = a.counts ? static_cast<double>(a.rows < a.num_groups ? a.rows : a.num_groups) : 1.0;
+    const double hbm = used * a.n * a.k / 6.4e6;
+    auto tiles = [&](double bm) {
+        if (!a.counts) return std::ceil(a.rows / bm) * n_tiles;
+        return std::max(used, a.rows / bm + used / 2) * n_tiles;
+    };
+    Choice best{0, 1};
+    double work = std::ceil(tiles(kBM) / sms) * (0.42 * k_blocks + 2.5), time = std::max(work, hbm);
+    for (int rows : {16, 32}) {
+        const double t = tiles(rows), block = rows == 16 ? 0.28 : 0.32;
+        for (int split : {1, 2, 4}) {
+            if (split > 1 && (t * split > (a.counts ? 0.6 : 0.87) * sms || split > k_blocks)) break;
+            const double w = split > 1 ? std::ceil(k_blocks / static_cast<double>(split)) * block + 2.5
+                                       : std::ceil(t / sms) * (block * k_blocks + 1.2);
+            const double us = std::max(w, hbm);
+            if (us < time || (us == time && (best.row_chunk == 0 || w < work))) {
+                best = {rows, split};
+                work = w;
+                time = us;
+            }
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -602,16 +558,11 @@ void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream) {
     p.k_blocks = (args.k + kBK - 1) / kBK;
     p.nb = (args.n + 127) / 128;
     p.error = gemm_error_word();
-    const CUtensorMap ta = make_tmap_2d(args.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, args.rows, args.k, args.lda, kBM, kBK);
-    const int64_t n_tiles = (args.n + kBN - 1) / kBN;
-    // At most this many tiles of bm rows, however the rows fall into groups.
-    auto most = [&](int64_t bm) { return ((args.rows + bm - 1) / bm + (args.counts ? args.num_groups : 0)) * n_tiles; };
-    const bool pair = use_pair(args, n_tiles);
-    const CUtensorMap tb =
-        make_tmap_2d(args.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, static_cast<uint64_t>(args.num_groups) * args.n, args.k,
-                     args.ldb, pair ? kBN / 2 : kBN, kBK);
-    if (pair) launch_epi<true>(ta, tb, p, most(2 * kBM), stream);
-    else launch_epi<false>(ta, tb, p, most(kBM), stream);
+    const Choice c = choose(args, p.k_blocks);
+    if (c.row_chunk) launch_few_rows(p, c.row_chunk, c.split, stream);
+    else if (!args.swiglu) launch<kEpiStore>(p, stream);
+    else if (!args.codes) launch<kEpiSwiGLU>(p, stream);
+    else launch<kEpiSwiGLUQuant>(p, stream);
 }
 
 void quant_fp8_blocks(const __nv_bfloat16* w, int64_t ld, int64_t rows, int64_t cols, uint8_t* codes, float* scales,

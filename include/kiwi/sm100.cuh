@@ -211,16 +211,6 @@ KIWI_DEV void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t
         : "memory");
 }
 
-/// mma_f8 over the tiles of a CTA pair (M = 256 across the pair).
-KIWI_DEV void mma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
 /// D[tmem] (+)= A[smem] * B[smem]^T, issued by one thread.
 KIWI_DEV void mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -287,6 +277,25 @@ KIWI_DEV void tmem_wait_32cols(uint32_t (&r)[32]) {
                  :
                  : "memory");
 }
+/// The same for 16 columns.
+KIWI_DEV void tmem_issue_16cols(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+KIWI_DEV void tmem_wait_16cols(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])
+                 :
+                 : "memory");
+}
 
 // ---- registers between warpgroups (whole warpgroup; the shares must not exceed the launch's total) ----
 
@@ -324,11 +333,31 @@ KIWI_DEV void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-/// Arrive on an mbarrier given by its cluster-window address without a
-/// cluster-scope release: for signals that hand over TMEM, which the tcgen05
-/// fences around them order, and no memory.
-KIWI_DEV void mbar_arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+/// mbar_wait whose success also orders what other CTAs of the cluster released
+/// to this barrier (their shared-memory writes) before what follows.
+KIWI_DEV bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t budget = 1u << 26) {
+    for (uint32_t i = 0; i < budget; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_addr(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+/// 16 bytes of the shared memory of CTA `rank` of this cluster, at the address of `p` in this one's.
+KIWI_DEV float4 ld_cluster_f32x4(const void* p, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(mapa(p, rank))
+                 : "memory");
+    return v;
 }
 
 /// 2-SM TMA load into this CTA's shared memory whose transaction bytes complete
@@ -367,15 +396,6 @@ KIWI_DEV void mma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, u
 KIWI_DEV void mma_commit_pair(uint32_t bar_cluster) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster)
                  : "memory");
-}
-
-/// mma_commit_pair to the barrier at the same offset in both CTAs of the pair, in one instruction.
-KIWI_DEV void mma_commit_both(uint64_t* bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            smem_addr(bar)),
-        "h"(static_cast<uint16_t>(3))
-        : "memory");
 }
 
 #endif  // __CUDACC__

@@ -52,7 +52,8 @@ def _close(got, ref, slack):
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 256, 128), (2, 7, 144), (33, 129, 112), (64, 1000, 256),
                                    (65, 384, 2064), (127, 255, 640), (129, 257, 384), (300, 640, 1040),
-                                   (1, 4096, 2048), (16, 1152, 7168), (700, 2048, 272)])
+                                   (1, 4096, 2048), (16, 1152, 7168), (700, 2048, 272),
+                                   (2000, 300, 272), (1500, 1003, 528), (3000, 512, 128), (200, 1111, 2064)])
 def test_dense_matches_64_bits(m, n, k):
     g = _gen(m * 7 + n)
     a, sa = _rows(g, m, k)
@@ -64,7 +65,7 @@ def test_dense_matches_64_bits(m, n, k):
     assert torch.equal(out, ops.fp8_gemm(a, sa, b, sb))  # nothing depends on the order of execution
 
 
-COUNTS = [[5], [0, 0, 130, 1], [256, 0, 77], [1] * 9, [0, 0], [64, 65, 128, 129], [1000, 3]]
+COUNTS = [[5], [0, 0, 130, 1], [256, 0, 77], [1] * 9, [0, 0], [64, 65, 128, 129], [1000, 3], [2000, 0, 1, 7000, 130]]
 
 
 @pytest.mark.parametrize("counts", COUNTS, ids=str)
@@ -100,7 +101,7 @@ def _swiglu(y, err):
     return h.flatten(1), (d + h.abs() * (16 + 2 * gate.abs()) * F32).flatten(1)
 
 
-@pytest.mark.parametrize("counts", [[5], [0, 130, 1], [3, 0, 260]], ids=str)
+@pytest.mark.parametrize("counts", [[5], [0, 130, 1], [3, 0, 260], [4000, 0, 3001]], ids=str)
 def test_swiglu_rows_come_back_quantised(counts):
     n, k = 768, 272
     rows = sum(counts) + 3
