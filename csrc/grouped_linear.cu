@@ -40,6 +40,7 @@
 #include "kiwi/gemm/group_table.cuh"
 #include "kiwi/gemm/grouped_gemm.hpp"
 #include "kiwi/gemm/grouped_linear.hpp"
+#include "kiwi/gemm/row_store.cuh"
 #include "kiwi/gemm/tensor_map.hpp"
 #include "kiwi/sm100.cuh"
 
@@ -62,7 +63,8 @@ struct Smem {
     static constexpr int kBBytes = kBN * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kTableOffset = kStages * kStageBytes;
-    static constexpr int kBarOffset = kTableOffset + static_cast<int>(round_up(sizeof(GroupTable), 16));
+    static constexpr int kStgOffset = kTableOffset + static_cast<int>(round_up(sizeof(GroupTable), 16));
+    static constexpr int kBarOffset = kStgOffset + kEpiThreads / 32 * kRowStoreBytes;
     static constexpr int kBytes = kBarOffset + 256 + 1024;  // barriers, TMEM slot, alignment slack
 };
 static_assert(Smem::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
@@ -74,36 +76,6 @@ struct Params {
     int k_blocks; // forward, dgrad: 64-wide blocks of the contraction
     uint32_t* error;
 };
-
-/// Eight fp32 values to eight columns of the result.
-template <typename T>
-__device__ __forceinline__ void put8(T* dst, const float* v, bool accumulate) {
-    if constexpr (sizeof(T) == 2) {
-        float f[8];
-        if (accumulate) {
-            ep::bf16x8_to_f32(*reinterpret_cast<const uint4*>(dst), f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] += v[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = v[i];
-        }
-        *reinterpret_cast<uint4*>(dst) = ep::f32x8_to_bf16(f);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            float4 o = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            if (accumulate) {
-                const float4 old = reinterpret_cast<const float4*>(dst)[j];
-                o.x += old.x;
-                o.y += old.y;
-                o.z += old.z;
-                o.w += old.w;
-            }
-            reinterpret_cast<float4*>(dst)[j] = o;
-        }
-    }
-}
 
 template <int MODE, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -121,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
     __shared__ int s_abort;
 
-    const int warp = threadIdx.x / 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform: the roles' addresses stay in uniform registers
     const int lane = threadIdx.x & 31;
     const int groups = p.a.num_groups;
     const int n_tiles = (p.n_cols + kBN - 1) / kBN;
@@ -217,9 +189,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp == 9) {
-        const uint32_t idesc =
+        // The whole warp walks the blocks and one elected lane issues, so that
+        // descriptors and addresses are warp-uniform.
+        constexpr uint32_t idesc =
             sm100::idesc_bf16_f32(kBM, kBN) | (kAMn ? sm100::kIdescAMn : 0u) | (kBMn ? sm100::kIdescBMn : 0u);
-        uint32_t it = 0;
+        const uint64_t a_desc0 = kAMn ? sm100::sw128_mnmajor_desc(smem) : sm100::sw128_kmajor_desc(smem);
+        const uint64_t b_desc0 = (kBMn ? sm100::sw128_mnmajor_desc(smem) : sm100::sw128_kmajor_desc(smem)) +
+                                 (Smem::kABytes >> 4);
+        const bool issuer = sm100::elect_one();
+        uint32_t it = 0, stage = 0, phase = 0;
         uint32_t n_acc = 0;  // accumulators started
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
@@ -228,26 +206,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int k_blocks = blocks_of(g);
             if (k_blocks == 0) continue;
             const uint32_t acc = n_acc & 1;
-            if (!sm100::mbar_wait(&tmem_empty[acc], ((n_acc >> 1) & 1) ^ 1)) {
-                fail();
-                break;
-            }
-            sm100::tc_fence_after();
+            ok = sm100::mbar_wait(&tmem_empty[acc], ((n_acc >> 1) & 1) ^ 1);
             const uint32_t d = tmem_base + acc * kBN;
-            for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                const uint32_t stage = it % kStages;
-                if (!sm100::mbar_wait(&full[stage], (it / kStages) & 1)) {
-                    fail();
-                    ok = false;
-                    break;
-                }
-                uint8_t* sa = smem + stage * Smem::kStageBytes;
-                uint8_t* sb = sa + Smem::kABytes;
+            for (int kb = 0; ok && kb < k_blocks; ++kb, ++it) {
+                ok = sm100::mbar_wait(&full[stage], phase);
+                if (!ok) break;
                 if constexpr (MODE == kWgrad) {
                     const int left = table.off[g + 1] - table.off[g] - kb * kBK;
                     if (left < kBK) {
                         // Rows past the group's: a box row is 128 contiguous bytes
                         // (the swizzle permutes within it).
+                        uint8_t* sa = smem + stage * Smem::kStageBytes;
                         for (int b = 0; b < (kBM + kBN) / 64; ++b) {
                             for (int o = left * 128 + lane * 16; o < kBox; o += 512) {
                                 *reinterpret_cast<uint4*>(sa + b * kBox + o) = make_uint4(0, 0, 0, 0);
@@ -258,9 +227,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 sm100::tc_fence_after();
-                if (lane == 0) {
-                    const uint64_t ad = kAMn ? sm100::sw128_mnmajor_desc(sa) : sm100::sw128_kmajor_desc(sa);
-                    const uint64_t bd = kBMn ? sm100::sw128_mnmajor_desc(sb) : sm100::sw128_kmajor_desc(sb);
+                const uint64_t ad = a_desc0 + stage * (Smem::kStageBytes >> 4);
+                const uint64_t bd = b_desc0 + stage * (Smem::kStageBytes >> 4);
+                if (issuer) {
 #pragma unroll
                     for (int kk = 0; kk < kBK / 16; ++kk) {
                         // 16 of K: 32 bytes along a swizzled row, or 16 rows of 128 bytes.
@@ -271,32 +240,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (kb == k_blocks - 1) sm100::mma_commit(&tmem_full[acc]);
                 }
                 __syncwarp();
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
             }
-            if (ok) ++n_acc;
+            if (!ok && issuer) fail();
+            ++n_acc;
         }
         // Nor may an MMA still write the TMEM that is freed below.
-        if (it > 0 && !sm100::mbar_wait(&empty[(it - 1) % kStages], ((it - 1) / kStages) & 1)) fail();
+        if (it > 0 && !sm100::mbar_wait(&empty[(it - 1) % kStages], ((it - 1) / kStages) & 1) && issuer) fail();
     } else {
         const int q = warp & 3;
         const int half = warp >> 2;
         const int row_in_tile = q * 32 + lane;
         T* const out = static_cast<T*>(p.a.out);
+        uint8_t* stg = smem + Smem::kStgOffset + warp * kRowStoreBytes;
         uint32_t n_acc = 0;
         for (int tile = blockIdx.x; tile < total_tiles && !aborted(); tile += gridDim.x) {
             int g, mt, nt;
             locate(tile, g, mt, nt);
-            int64_t row;
-            bool valid;
-            if constexpr (MODE == kWgrad) {
-                const int r = mt * kBM + row_in_tile;
-                row = static_cast<int64_t>(g) * p.m_cols + r;
-                valid = r < p.m_cols;
-            } else {
-                row = static_cast<int64_t>(table.off[g]) + mt * kBM + row_in_tile;
-                valid = row < table.off[g + 1];
-            }
+            const int64_t row = MODE == kWgrad
+                                    ? static_cast<int64_t>(g) * p.m_cols + mt * kBM + row_in_tile
+                                    : static_cast<int64_t>(table.off[g]) + mt * kBM + row_in_tile;
+            const int64_t r0 = row - lane;  // the warp's first row, and how many of its rows are the result's
+            const int64_t r_end = MODE == kWgrad ? static_cast<int64_t>(g + 1) * p.m_cols : table.off[g + 1];
+            const int rows = static_cast<int>(r_end - r0 < 32 ? r_end - r0 : 32);
             const int col0 = nt * kBN + half * (kBN / 2);
-            T* dst = out + row * p.a.ldo + col0;
             const int cols = p.n_cols - col0;  // a multiple of 64
             const bool have = blocks_of(g) != 0;
             const uint32_t acc = n_acc & 1;
@@ -307,8 +277,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             sm100::tc_fence_after();
             const uint32_t taddr =
                 tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN + static_cast<uint32_t>(half * (kBN / 2));
+            // A group without rows has a zero gradient, or adds nothing.
+            const bool store = rows > 0 && (have || !p.a.accumulate);
 #pragma unroll 1
-            for (int c = 0; c < kBN / 2; c += 32) {
+            for (int c = 0; c < kBN / 2 && c < cols; c += 32) {
                 float v[32];
                 if (have) {
                     sm100::tmem_ld_32cols(taddr + c, v);
@@ -316,9 +288,31 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0.f;
                 }
-                if (valid && c < cols && (have || !p.a.accumulate)) {
+                if (!store) continue;
+                T* dst = out + r0 * p.a.ldo + col0 + c;
+                if (sizeof(T) == 2 && !(MODE == kWgrad && p.a.accumulate)) {
+                    uint4 w[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) put8(dst + c + 8 * j, v + 8 * j, MODE == kWgrad && p.a.accumulate);
+                    for (int j = 0; j < 4; ++j) {
+                        float f[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) f[i] = v[8 * j + i];
+                        w[j] = ep::f32x8_to_bf16(f);
+                    }
+                    store_rows64(stg, w, reinterpret_cast<uint8_t*>(dst), p.a.ldo * 2, rows, 64, true);
+                } else if constexpr (MODE == kWgrad) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint4 w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float* f = v + 16 * h + 4 * j;
+                            w[j] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                              __float_as_uint(f[3]));
+                        }
+                        if (p.a.accumulate) add_rows16(stg, w, dst + 16 * h, p.a.ldo, rows);
+                        else store_rows64(stg, w, reinterpret_cast<uint8_t*>(dst + 16 * h), p.a.ldo * sizeof(T), rows, 64, true);
+                    }
                 }
             }
             if (have) {
@@ -331,8 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (MODE != kWgrad && p.a.zero_tail) {
             for (int64_t r = table.off[groups] + static_cast<int64_t>(blockIdx.x); r < p.a.rows; r += gridDim.x) {
                 for (int c = threadIdx.x * 8; c < p.n_cols; c += kEpiThreads * 8) {
-                    const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    put8(out + r * p.a.ldo + c, z, false);
+                    *reinterpret_cast<uint4*>(out + r * p.a.ldo + c) = make_uint4(0, 0, 0, 0);
                 }
             }
         }

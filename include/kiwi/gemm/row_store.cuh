@@ -1,6 +1,7 @@
 // Coalesced stores of an epilogue whose threads each hold a piece of one row.
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -40,6 +41,40 @@ __device__ __forceinline__ void store_rows64(uint8_t* stg, const uint4 (&w)[4], 
             const uint16_t x = *reinterpret_cast<const uint16_t*>(
                 stg + row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) * 16) + (lane & 7) * 2);
             if (lane * 2 < bytes) *reinterpret_cast<uint16_t*>(dst + row * ld_bytes + lane * 2) = x;
+        }
+    }
+    __syncwarp();
+}
+
+/// The same for 16 fp32 values a lane that are added to dst's rows, of bf16 or
+/// fp32 elements: one addition in fp32 and one rounding each.
+template <typename T>
+__device__ __forceinline__ void add_rows16(uint8_t* stg, const uint4 (&w)[4], T* dst, int64_t ld, int rows) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stg + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = w[j];
+    __syncwarp();
+    const int piece = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2);
+        if (row >= rows) continue;
+        const float4 x = *reinterpret_cast<const float4*>(stg + row * 64 + ((piece ^ ((row >> 1) & 3)) * 16));
+        T* at = dst + row * ld + piece * 4;
+        if constexpr (sizeof(T) == 4) {
+            float4 o = *reinterpret_cast<const float4*>(at);
+            o.x += x.x;
+            o.y += x.y;
+            o.z += x.z;
+            o.w += x.w;
+            *reinterpret_cast<float4*>(at) = o;
+        } else {
+            __nv_bfloat162 o[2];
+            *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(at);
+            const float2 lo = __bfloat1622float2(o[0]), hi = __bfloat1622float2(o[1]);
+            o[0] = __floats2bfloat162_rn(lo.x + x.x, lo.y + x.y);
+            o[1] = __floats2bfloat162_rn(hi.x + x.z, hi.y + x.w);
+            *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(o);
         }
     }
     __syncwarp();
