@@ -4,6 +4,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/pybind11.h>
+#include <pybind11/stl.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -320,7 +321,8 @@ torch::Tensor swiglu_py(torch::Tensor y, OptTensor row_scale) {
     return h;
 }
 
-py::tuple swiglu_grad_py(torch::Tensor dh, torch::Tensor y, OptTensor row_scale, bool need_scale_grad) {
+std::pair<torch::Tensor, OptTensor> swiglu_grad(torch::Tensor dh, torch::Tensor y, OptTensor row_scale,
+                                                bool need_scale_grad) {
     check_swiglu(y, row_scale);
     check_bf16_rows(dh, y.device(), "dh");
     require(dh.size(0) == y.size(0) && dh.size(1) * 2 == y.size(1), "dh must be [rows, F] for y [rows, 2F]");
@@ -334,8 +336,69 @@ py::tuple swiglu_grad_py(torch::Tensor dh, torch::Tensor y, OptTensor row_scale,
                          row_scale ? row_scale->data_ptr<float>() : nullptr,
                          reinterpret_cast<__nv_bfloat16*>(dy.data_ptr()), ds ? ds->data_ptr<float>() : nullptr,
                          y.size(0), static_cast<int>(dh.size(1)), cur_stream());
-    return py::make_tuple(dy, ds);
+    return {dy, ds};
 }
+
+// ---- autograd (CUDA tensors; the CPU restatements have their own in Python) ----
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+/// Passes a gradient on, and refuses to be differentiated: the gradients of this
+/// file are once differentiable.  Its other arguments are what the gradient was
+/// computed from.
+struct OnceDifferentiable : torch::autograd::Function<OnceDifferentiable> {
+    static torch::Tensor forward(AutogradContext*, torch::Tensor grad, torch::Tensor, torch::Tensor, OptTensor) {
+        return grad.view_as(grad);
+    }
+    static variable_list backward(AutogradContext*, variable_list) {
+        TORCH_CHECK(false, "the gradients of grouped_linear and swiglu are once differentiable");
+    }
+    static torch::Tensor mark(const torch::Tensor& grad, const torch::Tensor& a, const torch::Tensor& b,
+                              const OptTensor& c = std::nullopt) {
+        return grad.defined() && torch::GradMode::is_enabled() ? apply(grad, a, b, c) : grad;
+    }
+};
+
+struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
+    static torch::Tensor forward(AutogradContext* ctx, torch::Tensor x, torch::Tensor w, torch::Tensor counts) {
+        ctx->save_for_backward({x, w, counts});
+        at::AutoDispatchBelowADInplaceOrView below;
+        return linear_forward_py(x, w, counts, std::nullopt);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const torch::Tensor &x = saved[0], &w = saved[1], &counts = saved[2], &dy = grads[0];
+        torch::Tensor dx, dw;
+        if (dy.defined()) {
+            at::AutoDispatchBelowADInplaceOrView below;
+            if (ctx->needs_input_grad(0)) dx = linear_dgrad_py(dy, w, counts, std::nullopt);
+            if (ctx->needs_input_grad(1)) dw = linear_wgrad_py(dy, x, counts, std::nullopt, false);
+        }
+        return {OnceDifferentiable::mark(dx, dy, w), OnceDifferentiable::mark(dw, dy, x), torch::Tensor()};
+    }
+};
+
+struct SwiGLU : torch::autograd::Function<SwiGLU> {
+    static torch::Tensor forward(AutogradContext* ctx, torch::Tensor y, OptTensor row_scale) {
+        ctx->save_for_backward({y, row_scale ? *row_scale : torch::Tensor()});
+        at::AutoDispatchBelowADInplaceOrView below;
+        return swiglu_py(y, row_scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const torch::Tensor &y = saved[0], &s = saved[1], &dh = grads[0];
+        if (!dh.defined()) return {torch::Tensor(), torch::Tensor()};
+        std::pair<torch::Tensor, OptTensor> r;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            r = swiglu_grad(dh, y, s.defined() ? OptTensor(s) : std::nullopt, s.defined() && ctx->needs_input_grad(1));
+        }
+        const OptTensor scale = s.defined() ? OptTensor(s) : std::nullopt;
+        return {OnceDifferentiable::mark(r.first, dh, y, scale),
+                r.second ? OnceDifferentiable::mark(*r.second, dh, y, scale) : torch::Tensor()};
+    }
+};
 
 /// Reads and clears a device's error word (waits for the current stream).
 int64_t gemm_error(int64_t device) {
@@ -367,15 +430,20 @@ void register_expert_ops(py::module_& m) {
           py::arg("out") = py::none(), "The experts' SwiGLU FFN on FP8 rows and weights (two launches).");
     o.def("quant_fp8_weights", &quant_fp8_weights_py, py::arg("w"),
           "128x128 FP8 e4m3 quantisation of a bf16 matrix: (codes, fp32 scales).");
-    o.def("grouped_linear", &linear_forward_py, py::arg("x"), py::arg("w"), py::arg("counts"),
-          py::arg("out") = py::none(), "y = x . w[g]^T for each group's rows.");
+    o.def("grouped_linear", [](torch::Tensor x, torch::Tensor w, torch::Tensor counts) {
+        return GroupedLinear::apply(x, w, counts);
+    }, py::arg("x"), py::arg("w"), py::arg("counts"), "y = x . w[g]^T for each group's rows; differentiable.");
+    o.def("grouped_linear_out", [](torch::Tensor x, torch::Tensor w, torch::Tensor counts, torch::Tensor out) {
+        return linear_forward_py(x, w, counts, out);
+    }, py::arg("x"), py::arg("w"), py::arg("counts"), py::arg("out"), "The same into out; not differentiable.");
     o.def("grouped_linear_dgrad", &linear_dgrad_py, py::arg("dy"), py::arg("w"), py::arg("counts"),
           py::arg("out") = py::none(), "dx = dy . w[g] for each group's rows.");
     o.def("grouped_linear_wgrad", &linear_wgrad_py, py::arg("dy"), py::arg("x"), py::arg("counts"),
           py::arg("out") = py::none(), py::arg("accumulate") = false, "dw[g] (+)= dy^T . x over each group's rows.");
-    o.def("swiglu", &swiglu_py, py::arg("y"), py::arg("row_scale") = py::none(),
-          "row_scale * silu(gate) * up of rows in blocks of 128 gate and 128 up columns.");
-    o.def("swiglu_grad", &swiglu_grad_py, py::arg("dh"), py::arg("y"), py::arg("row_scale") = py::none(),
+    o.def("swiglu", [](torch::Tensor y, OptTensor row_scale) { return SwiGLU::apply(y, row_scale); }, py::arg("y"),
+          py::arg("row_scale") = py::none(),
+          "row_scale * silu(gate) * up of rows in blocks of 128 gate and 128 up columns; differentiable.");
+    o.def("swiglu_grad", &swiglu_grad, py::arg("dh"), py::arg("y"), py::arg("row_scale") = py::none(),
           py::arg("need_scale_grad") = false, "(dy, drow_scale or None) of swiglu.");
     o.def("gemm_error", &gemm_error, py::arg("device"), "Reads and clears the products' error word of a device.");
 }

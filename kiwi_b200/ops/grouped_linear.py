@@ -63,10 +63,6 @@ def _fill(out, res, total):
 
 
 def _forward(x, w, counts, out=None):
-    if x.is_cuda:
-        from .. import native
-
-        return native().ops.grouped_linear(x, w, counts, out)
     _check_counts(counts)
     if w.dtype != torch.bfloat16 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.shape[0] % counts.numel():
         raise ValueError("w must be bf16 [groups * N, K] with x's K")
@@ -127,7 +123,7 @@ def grouped_linear_wgrad(dy, x, counts, out=None, accumulate=False):
     return out.copy_(out.float() + res if accumulate else res)
 
 
-class _GroupedLinear(torch.autograd.Function):
+class _GroupedLinear(torch.autograd.Function):  # CPU tensors; the native op has its own
     @staticmethod
     def forward(ctx, x, w, counts):
         ctx.save_for_backward(x, w, counts)
@@ -149,8 +145,12 @@ def grouped_linear(x, w, counts, out=None):
     if out is not None:
         if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
             raise ValueError("out is not differentiable: leave it out, or call under torch.no_grad()")
-        return _forward(x, w, counts, out)
-    return _GroupedLinear.apply(x, w, counts)
+    if x.is_cuda:
+        from .. import native
+
+        o = native().ops
+        return o.grouped_linear(x, w, counts) if out is None else o.grouped_linear_out(x, w, counts, out)
+    return _GroupedLinear.apply(x, w, counts) if out is None else _forward(x, w, counts, out)
 
 
 def _swiglu_halves(y):
@@ -187,14 +187,10 @@ def swiglu_grad(dh, y, row_scale=None, need_scale_grad=None):
     return dy, ((d * g * sig * u).sum(1) if need else None)
 
 
-class _SwiGLU(torch.autograd.Function):
+class _SwiGLU(torch.autograd.Function):  # CPU tensors; the native op has its own
     @staticmethod
     def forward(ctx, y, row_scale):
         ctx.save_for_backward(y, row_scale)
-        if y.is_cuda:
-            from .. import native
-
-            return native().ops.swiglu(y, row_scale)
         _check_swiglu(y, row_scale)
         g, u = _swiglu_halves(y.float())
         h = g * torch.sigmoid(g) * u
@@ -210,6 +206,10 @@ class _SwiGLU(torch.autograd.Function):
 def swiglu(y, row_scale=None):
     """bf16 [rows, F] of y [rows, 2F] (blocks of 128 gate and 128 up columns),
     times ``row_scale`` (fp32 [rows]); differentiable in both."""
+    if y.is_cuda:
+        from .. import native
+
+        return native().ops.swiglu(y, row_scale)
     return _SwiGLU.apply(y, row_scale)
 
 

@@ -277,6 +277,23 @@ def test_ffn_gradients_against_differences():
         assert abs(float((got.double() * v).sum() - diff)) <= 4 * BF16 * float(want.norm() * v.norm())
 
 
+def test_gradients_are_once_differentiable_and_only_those_asked_for():
+    x, w, dy, cnt = _data(_gen(16), [9, 5], 128, 256)
+    x.requires_grad_()
+    y = ops.grouped_linear(x, w, cnt)
+    dx, = torch.autograd.grad(y, x, dy.clone().requires_grad_(), create_graph=True)
+    assert torch.equal(dx, ops.grouped_linear_dgrad(dy, w, cnt))
+    with pytest.raises(RuntimeError, match="once differentiable"):
+        dx.float().sum().backward()
+    s = torch.ones(14, device="cuda", requires_grad=True)
+    ds, = torch.autograd.grad(ops.swiglu(x.detach(), s).float().sum(), s, create_graph=True)
+    with pytest.raises(RuntimeError, match="once differentiable"):
+        ds.sum().backward()
+    assert not ops.grouped_linear(x.detach(), w, cnt).requires_grad
+    with torch.no_grad():
+        assert not ops.swiglu(x).requires_grad
+
+
 def test_captured_step_follows_counts_and_data():
     """Forward and both gradients in one graph, next to live eager graphs of other leaves."""
     counts, n, k = [20, 30], 128, 128
