@@ -5,7 +5,7 @@
 // of gate and one of up), and up to ROWS rows of the group its N operand.  What
 // counts here is reading the weights once at the memory's rate: a stage holds
 // 32 KB of weights and only ROWS * 128 bytes of rows, an accumulator 2 * ROWS
-// TMEM columns, so that four of them are in flight and the drain (one FMA per
+// TMEM columns, so that five of them are in flight and the drain (one FMA per
 // weight row and token) hides.
 //
 // Where the tiles do not fill the GPU, a cluster of SPLIT CTAs shares a tile
@@ -43,7 +43,8 @@ namespace {
 
 constexpr int kThreads = 352;
 constexpr int kDrainThreads = 256;
-constexpr int kRing = 4;  // stages, and TMEM accumulators
+// Stages, and TMEM accumulators: the most that fit (4 read weights 4 % slower).
+constexpr int kRing = 5;
 
 template <int ROWS>
 struct Smem {
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::tma_prefetch_desc(&tmap_a);
         sm100::tma_prefetch_desc(&tmap_b);
     }
-    if (warp == 9) sm100::tmem_alloc(tmem_slot, kRing * kCols);
+    if (warp == 9) sm100::tmem_alloc(tmem_slot, 8 * kCols);
     build_group_table(table, p.a.counts, groups, p.a.rows, ROWS, n_tiles, p.error);
     sm100::tc_fence_before();
     __syncthreads();
@@ -126,6 +127,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = table.tiles[groups];
 
+    auto next = [](uint32_t& slot, uint32_t& phase) {
+        if (++slot == kRing) {
+            slot = 0;
+            phase ^= 1;
+        }
+    };
     auto aborted = [&]() { return *reinterpret_cast<volatile int*>(&s_abort) != 0; };
     auto fail = [&]() {
         *reinterpret_cast<volatile int*>(&s_abort) = 1;
@@ -134,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 8) {
         if (lane == 0) {
-            uint32_t issued = 0;
+            uint32_t issued = 0, stage = 0, phase = 0;
             bool ok = true;
             for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
                 int g, mt, nt;
@@ -142,8 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int row0 = table.off[g] + mt * ROWS;
                 const int brow0 = g * p.a.n + nt * kBN;
                 for (int kb = kb0; kb < kb1; ++kb, ++issued) {
-                    const uint32_t stage = issued % kRing;
-                    if (!sm100::mbar_wait(&done[stage], ((issued / kRing) & 1) ^ 1)) {
+                    if (!sm100::mbar_wait(&done[stage], phase ^ 1)) {
                         fail();
                         ok = false;
                         break;
@@ -152,6 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sm100::mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
                     sm100::tma_load_2d(sw, &tmap_b, &full[stage], kb * kBK, brow0);
                     sm100::tma_load_2d(sw + S::kWBytes, &tmap_a, &full[stage], kb * kBK, row0);
+                    next(stage, phase);
                 }
             }
             // No load may still be in flight when this CTA's shared memory goes away.
@@ -163,11 +170,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t idesc = sm100::idesc_e4m3_f32(128, ROWS);
         const uint64_t desc0 = sm100::sw128_kmajor_desc(smem);
         const bool issuer = sm100::elect_one();
-        uint32_t it = 0;
+        uint32_t it = 0, slot = 0, phase = 0;
         bool ok = true;
         for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t slot = it % kRing, phase = (it / kRing) & 1;
                 ok = sm100::mbar_wait(&drained[slot], phase ^ 1) && sm100::mbar_wait(&full[slot], phase);
                 if (!ok) {
                     if (issuer) fail();
@@ -188,12 +194,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sm100::mma_commit(&done[slot]);
                 }
                 __syncwarp();
+                next(slot, phase);
             }
         }
         // Nor may an MMA still write the TMEM that is freed below.
         if (it > 0 && !sm100::mbar_wait(&done[(it - 1) % kRing], ((it - 1) / kRing) & 1) && issuer) fail();
     } else if (warp == 10) {
-        uint32_t it = 0;
+        uint32_t slot = 0, phase = 0;
         bool ok = true;
         for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
             int g, mt, nt;
@@ -204,15 +211,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float* sb0 = p.a.b_scale + (static_cast<int64_t>(g) * p.nb + 2 * nt) * p.k_blocks;
             const float* sb1 = 2 * nt + 1 < p.nb ? sb0 + p.k_blocks : sb0;
             float a = __ldg(sa + kb0), b0 = __ldg(sb0 + kb0), b1 = __ldg(sb1 + kb0);
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 const float v0 = a * b0, v1 = a * b1;
                 if (kb + 1 < kb1) {
                     a = __ldg(sa + kb + 1);
                     b0 = __ldg(sb0 + kb + 1);
                     b1 = __ldg(sb1 + kb + 1);
                 }
-                const uint32_t slot = it % kRing;
-                if (!sm100::mbar_wait(&drained[slot], ((it / kRing) & 1) ^ 1)) {
+                if (!sm100::mbar_wait(&drained[slot], phase ^ 1)) {
                     if (lane == 0) fail();
                     ok = false;
                     break;
@@ -223,12 +229,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&done[slot]);
+                next(slot, phase);
             }
         }
     } else if (warp < 8) {
         const int q = warp & 3;
         const int mb = warp >> 2;  // weight block: with SwiGLU gate or up
-        uint32_t it = 0;
+        uint32_t slot = 0, phase = 0;
         uint32_t n_sum = 0;  // tiles whose sums were shared
         bool ok = true;
         for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step, ++n_sum) {
@@ -238,9 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < ROWS / 2; ++i) acc[i] = 0;
 #pragma unroll 1
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t slot = it % kRing;
-                if (!sm100::mbar_wait(&done[slot], (it / kRing) & 1)) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!sm100::mbar_wait(&done[slot], phase)) {
                     fail();
                     ok = false;
                     break;
@@ -266,6 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sm100::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&drained[slot]);
+                next(slot, phase);
             }
             if (!ok) break;
             const int64_t row0 = static_cast<int64_t>(table.off[g]) + mt * ROWS;
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (split > 1) sm100::cluster_sync();  // no CTA leaves while another may read its sums
     sm100::tc_fence_after();
-    if (warp == 9) sm100::tmem_dealloc(tmem_base, kRing * kCols);
+    if (warp == 9) sm100::tmem_dealloc(tmem_base, 8 * kCols);
 }
 
 template <int EPI, int ROWS>
