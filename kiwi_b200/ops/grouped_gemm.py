@@ -158,9 +158,17 @@ class ExpertFFN:
     hidden buffer and GEMM2 with the per-row scale (the routing weight) and
     returns the bf16 rows [max_rows, H] (the first ``sum(counts)`` valid).
     ``weight_layout="blocked"`` (the default) gives both GEMMs blocked copies
-    of the weights (:func:`block_weights`; same result, faster weight loads)."""
+    of the weights (:func:`block_weights`; same result, faster weight loads).
 
-    def __init__(self, w13, w2, num_experts, max_rows, weight_layout="blocked"):
+    ``weight_format="fp8"`` keeps the weights as e4m3 codes with 128 x 128 block
+    scales (:func:`kiwi_b200.ops.quant_fp8_weights`; half the memory, row-major
+    whatever ``weight_layout``) and runs both products in FP8
+    (:func:`kiwi_b200.ops.expert_ffn_fp8`).  H and F are then multiples of 128,
+    and each call quantises the input buffer's rows, or takes rows that are FP8
+    already: ``ffn(counts, row_scale, rows=(codes, scales))`` with 1 x 128 scales,
+    as the FP8 dispatch delivers them, returns as many rows as those have."""
+
+    def __init__(self, w13, w2, num_experts, max_rows, weight_layout="blocked", weight_format="bf16"):
         e = int(num_experts)
         if w13.shape[0] % (2 * e) or w2.shape[0] % e:
             raise ValueError("w13 must be [E * 2F, H] and w2 [E * H, F]")
@@ -169,24 +177,57 @@ class ExpertFFN:
             raise ValueError(f"w2 must be [{e * hidden}, {ffn}]")
         if ffn % 128:
             raise ValueError("the SwiGLU epilogue needs F to be a multiple of 128")
+        if weight_format not in ("bf16", "fp8"):
+            raise ValueError("weight_format must be 'bf16' or 'fp8'")
+        if weight_format == "fp8" and hidden % 128:
+            raise ValueError("FP8 weights need H to be a multiple of 128")
         dev = w13.device
         self.num_experts, self.hidden, self.ffn, self.max_rows = e, hidden, ffn, int(max_rows)
+        self.weight_format = weight_format
         rows = max(self.max_rows, 1)
         self._a = torch.zeros(rows, hidden, dtype=torch.bfloat16, device=dev)
-        self._h = torch.zeros(rows, ffn, dtype=torch.bfloat16, device=dev)
         self._y = torch.zeros(rows, hidden, dtype=torch.bfloat16, device=dev)
+        if weight_format == "fp8":
+            from .fp8_gemm import quant_fp8_weights
+
+            self.w13, self.w13_scale = quant_fp8_weights(w13)
+            self.w2, self.w2_scale = quant_fp8_weights(w2)
+            return
+        self._h = torch.zeros(rows, ffn, dtype=torch.bfloat16, device=dev)
         self.gemm1 = GroupedGemm(self._a, w13, e, b_layout=weight_layout)
         self.gemm2 = GroupedGemm(self._h, w2, e, b_layout=weight_layout)
+        # The GEMMs' own weights (on CUDA, blocked copies of the row-major inputs).
+        self.w13, self.w2 = self.gemm1.b, self.gemm2.b
 
     def input_buffer(self):
         return self._a
 
-    def __call__(self, counts, row_scale=None):
+    def __call__(self, counts, row_scale=None, rows=None):
+        if self.weight_format == "fp8":
+            from .fp8_gemm import expert_ffn_fp8
+            from .quant import quant_fp8
+
+            codes, scales = quant_fp8(self._a) if rows is None else rows
+            n = codes.shape[0]
+            if n > self._y.shape[0]:
+                raise ValueError(f"{n} rows for an op of {self.max_rows}")
+            y = self._y[:n]
+            expert_ffn_fp8(codes, scales, self.w13, self.w13_scale, self.w2, self.w2_scale, counts,
+                           row_scale=None if row_scale is None else row_scale[:n], out=y)
+            return y
+        if rows is not None:
+            raise ValueError("FP8 rows need weight_format='fp8'")
         self.gemm1(counts, self._h, swiglu=True)
         self.gemm2(counts, self._y, swiglu=False, row_scale=row_scale)
         return self._y
 
     def check(self):
+        if self.weight_format == "fp8":
+            if self._a.is_cuda:
+                from .fp8_gemm import check_gemm
+
+                check_gemm(self._a.device)
+            return
         self.gemm1.check()
         self.gemm2.check()
 

@@ -336,9 +336,14 @@ class CollectiveMoE:
     the token goes back, so one row per (token, destination rank) travels each
     way.  The experts run :class:`kiwi_b200.ops.ExpertFFN` (the tcgen05 grouped
     GEMM on CUDA tensors, its fp32 reference in CPU processes).  Collective:
-    every rank of the group calls forward in the same order."""
+    every rank of the group calls forward in the same order.
 
-    def __init__(self, cfg, group=None, max_tokens=None, weights=None, device=None, combine_dtype=torch.bfloat16):
+    ``weight_format="fp8"`` runs the experts in FP8 (block-scaled weights): rows
+    that were dispatched in FP8 go into the products as they arrive, others are
+    quantised first."""
+
+    def __init__(self, cfg, group=None, max_tokens=None, weights=None, device=None, combine_dtype=torch.bfloat16,
+                 weight_format="bf16"):
         if cfg.quant not in ("none", "fp8", "nvfp4"):
             raise ValueError("CollectiveMoE carries bf16 ('none'), FP8 or NVFP4 rows")
         world = kdist.world_size(group)
@@ -354,9 +359,10 @@ class CollectiveMoE:
         if weights is None:
             weights = moe_model.local_expert_weights(cfg, self.rank, self.world, self.device)
         max_pairs = self.world * self.max_tokens * min(cfg.topk, self.experts_per_rank)
-        self.experts = ExpertFFN(weights[0], weights[1], self.experts_per_rank, max_pairs)
-        # The expert GEMMs' own weights (on CUDA, blocked copies of the row-major inputs).
-        self.w13, self.w2 = self.experts.gemm1.b, self.experts.gemm2.b
+        self.experts = ExpertFFN(weights[0], weights[1], self.experts_per_rank, max_pairs,
+                                 weight_format=weight_format)
+        # The experts' own weights (on CUDA, blocked or FP8 copies of the row-major inputs).
+        self.w13, self.w2 = self.experts.w13, self.experts.w2
         self._scale = torch.zeros(max(max_pairs, 1), dtype=torch.float32, device=self.device)
 
     def forward(self, x, router_logits):
@@ -370,7 +376,10 @@ class CollectiveMoE:
         """Same layer with precomputed routing (idx [T, k] global expert ids, w [T, k])."""
         rows, rw, scales, ridx, _ = self.op.dispatch(x, w, None, idx)
         n, h = rows.shape
-        if self.cfg.quant == "nvfp4":  # e2m1 codes x block scales -> operand rows
+        fp8_rows = self.experts.weight_format == "fp8" and self.cfg.quant == "fp8"
+        if fp8_rows:  # codes and 1x128 scales are the products' operands
+            h = self.cfg.hidden
+        elif self.cfg.quant == "nvfp4":  # e2m1 codes x block scales -> operand rows
             h = self.cfg.hidden
             rows = moe_model.dequant_nvfp4(rows, scales)
         elif scales is not None:  # FP8 codes x 1x128 scales -> operand rows
@@ -382,9 +391,12 @@ class CollectiveMoE:
         r, s, e = r[order], s[order], e[order]
         p = r.numel()
         counts = torch.bincount(e, minlength=self.experts_per_rank).to(torch.int32)
-        self.experts.input_buffer()[:p].copy_(rows[r])
         self._scale[:p].copy_(rw[r, s])
-        y = self.experts(counts, self._scale)
+        if fp8_rows:
+            y = self.experts(counts, self._scale, rows=(rows[r], scales[r]))
+        else:
+            self.experts.input_buffer()[:p].copy_(rows[r])
+            y = self.experts(counts, self._scale)
         partial = torch.zeros(n, h, dtype=torch.float32, device=self.device)
         if p:
             partial.index_add_(0, r, y[:p].float())

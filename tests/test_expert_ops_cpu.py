@@ -171,3 +171,61 @@ def test_grouped_linear_refusals():
     for f in bad:
         with pytest.raises(ValueError):
             f()
+
+
+# ---------------------------------------------------------------- the layers that use them
+
+
+@pytest.mark.parametrize("quant", ["none", "fp8", "nvfp4"])
+def test_fp8_experts_in_the_collective_layer(quant):
+    """The layer with FP8 experts equals its own pieces: the dispatched rows, FP8
+    weights, the FFN's reference and the routing-weighted sum."""
+    from kiwi_b200.models import moe
+    from kiwi_b200.parallel.ep_collective import CollectiveMoE
+
+    cfg = moe.MoEConfig(hidden=256, ffn=128, num_experts=3, topk=2, tokens_per_rank=20, quant=quant, name="t")
+    layer = CollectiveMoE(cfg, device="cpu", weight_format="fp8")
+    assert layer.w13.dtype == torch.float8_e4m3fn
+    x, logits = moe.synthetic_inputs(cfg, 0, "cpu", tokens=17)
+    out = layer(x, logits)
+    layer.check()
+    idx, w = moe.route_reference(logits, cfg.topk)
+    codes, scales = moe.quant_fp8_codes(x) if quant == "fp8" else moe.quant_fp8_codes(
+        moe.dispatch_reference(x, quant).bfloat16())
+    ref = torch.zeros(17, 256)
+    for e in range(3):
+        t, s = (idx == e).nonzero(as_tuple=True)
+        a, b, c = moe.expert_weights(cfg, e, "cpu")
+        w13, s13 = ops.quant_fp8_weights(moe.interleave_gate_up(a, b))
+        w2, s2 = ops.quant_fp8_weights(c)
+        y = ops.expert_ffn_fp8(codes[t], scales[t], w13, s13, w2, s2, [len(t)], row_scale=w[t, s].float().contiguous())
+        ref.index_add_(0, t, y.float())
+    # The layer sums bf16 rows in fp32 and rounds once more.
+    assert bool(((out.float() - ref).abs() <= BF16 * ref.abs() + 1e-6).all())
+
+
+def test_fp8_expert_ffn_object():
+    from kiwi_b200.models import moe
+
+    cfg = moe.MoEConfig(hidden=256, ffn=128, num_experts=3, topk=1, tokens_per_rank=8, quant="none", name="t")
+    w13, w2 = moe.local_expert_weights(cfg, 0, 1, "cpu")
+    ffn = ops.ExpertFFN(w13, w2, 3, 16, weight_format="fp8")
+    x = torch.randn(10, 256).bfloat16()
+    ffn.input_buffer()[:10].copy_(x)
+    counts, scale = torch.tensor([4, 0, 6]), torch.rand(16)
+    y = ffn(counts, scale)
+    assert tuple(y.shape) == (16, 256)
+    rows = ops.quant_fp8(x)
+    want = ops.expert_ffn_fp8(*rows, ffn.w13, ffn.w13_scale, ffn.w2, ffn.w2_scale, counts, row_scale=scale[:10])
+    assert torch.equal(y[:10], want) and torch.equal(ffn(counts, scale, rows=rows), want)
+    ffn.check()
+    # And near the bf16 experts: e4m3 rows, weights and hidden rows are each off
+    # by at most 2^-4 of a value, which a norm over many sees well below 3 * 2^-4.
+    ref = ops.ExpertFFN(w13, w2, 3, 16)
+    ref.input_buffer()[:10].copy_(x)
+    full = ref(counts, scale)[:10].float()
+    assert (want.float() - full).norm() <= 3 * 2.0 ** -4 * full.norm()
+    for bad in (lambda: ops.ExpertFFN(w13, w2, 3, 16, weight_format="int8"), lambda: ref(counts, scale, rows=rows),
+                lambda: ffn(counts, scale, rows=ops.quant_fp8(torch.zeros(17, 256).bfloat16()))):
+        with pytest.raises(ValueError):
+            bad()

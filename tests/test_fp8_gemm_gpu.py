@@ -334,3 +334,52 @@ def test_refusals():
             f()
     assert tuple(ops.fp8_gemm(a[:0], sa[:0], b, sb).shape) == (0, 512)
     ops.check_gemm()
+
+
+@pytest.mark.parametrize("quant", ["none", "fp8"])
+def test_fp8_experts_in_the_collective_layer(quant):
+    """The layer with FP8 experts equals its own pieces: dispatched rows, FP8
+    weights, each expert's FFN and the routing-weighted sum."""
+    from kiwi_b200.models import moe
+    from kiwi_b200.parallel.ep_collective import CollectiveMoE
+
+    cfg = moe.MoEConfig(hidden=512, ffn=256, num_experts=8, topk=2, tokens_per_rank=64, quant=quant, name="t")
+    layer = CollectiveMoE(cfg, weight_format="fp8")
+    for step in range(2):
+        t = 64 - 20 * step
+        x, logits = moe.synthetic_inputs(cfg, 0, "cuda", tokens=t, step=step)
+        out = layer(x, logits)
+        layer.check()
+        idx, w = ops.route_topk(logits, cfg.topk)
+        codes, scales = ops.quant_fp8(x)
+        ref = torch.zeros(t, 512, device="cuda")
+        for e in range(8):
+            r, s = (idx == e).nonzero(as_tuple=True)
+            a, b, c = moe.expert_weights(cfg, e, "cuda")
+            w13, s13 = ops.quant_fp8_weights(moe.interleave_gate_up(a, b))
+            w2, s2 = ops.quant_fp8_weights(c)
+            y = ops.expert_ffn_fp8(codes[r], scales[r], w13, s13, w2, s2, [len(r)], row_scale=w[r, s].contiguous())
+            ref.index_add_(0, r, y.float())
+        # bf16 rows of this comparison may be rounded from sums in another order
+        # (the kernels split K by the number of rows): one bf16 step each way.
+        assert bool(((out.float() - ref).abs() <= 4 * BF16 * ref.abs() + 2 * BF16 * ref.abs().max()).all())
+        assert (out.float() - ref).norm() <= 2 * BF16 * ref.norm()
+
+
+def test_fp8_expert_ffn_object():
+    from kiwi_b200.models import moe
+
+    cfg = moe.MoEConfig(hidden=256, ffn=128, num_experts=3, topk=1, tokens_per_rank=8, quant="none", name="t")
+    w13, w2 = moe.local_expert_weights(cfg, 0, 1, "cuda")
+    ffn = ops.ExpertFFN(w13, w2, 3, 16, weight_format="fp8")
+    x = torch.randn(10, 256, device="cuda").bfloat16()
+    ffn.input_buffer()[:10].copy_(x)
+    counts, scale = torch.tensor([4, 0, 6], device="cuda"), torch.rand(16, device="cuda")
+    rows = ops.quant_fp8(x)
+    want = ops.expert_ffn_fp8(*rows, ffn.w13, ffn.w13_scale, ffn.w2, ffn.w2_scale, counts, row_scale=scale[:10])
+    y = ffn(counts, scale).clone()
+    assert tuple(y.shape) == (16, 256) and (y[:10].float() - want.float()).norm() <= BF16 * want.float().norm()
+    assert torch.equal(ffn(counts, scale, rows=rows), want)
+    ffn.check()
+    with pytest.raises(ValueError):
+        ffn(counts, scale, rows=ops.quant_fp8(torch.zeros(17, 256, device="cuda").bfloat16()))
