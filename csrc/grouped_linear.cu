@@ -138,6 +138,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         return MODE == kWgrad ? (table.off[g + 1] - table.off[g] + kBK - 1) / kBK : p.k_blocks;
     };
 
+    // A tile with at most 64 rows of its group left runs M = 64 MMAs: half the
+    // tensor work, the same sums.  Its row 16 q + i is in TMEM lane 32 q + i.
+    auto half_tile = [&](int g, int mt) {
+        return MODE != kWgrad && table.off[g + 1] - table.off[g] - mt * kBM <= 64;
+    };
+
     auto aborted = [&]() { return *reinterpret_cast<volatile int*>(&s_abort) != 0; };
     auto fail = [&]() {
         *reinterpret_cast<volatile int*>(&s_abort) = 1;
@@ -191,8 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 9) {
         // The whole warp walks the blocks and one elected lane issues, so that
         // descriptors and addresses are warp-uniform.
-        constexpr uint32_t idesc =
-            sm100::idesc_bf16_f32(kBM, kBN) | (kAMn ? sm100::kIdescAMn : 0u) | (kBMn ? sm100::kIdescBMn : 0u);
+        constexpr uint32_t majors = (kAMn ? sm100::kIdescAMn : 0u) | (kBMn ? sm100::kIdescBMn : 0u);
         const uint64_t a_desc0 = kAMn ? sm100::sw128_mnmajor_desc(smem) : sm100::sw128_kmajor_desc(smem);
         const uint64_t b_desc0 = (kBMn ? sm100::sw128_mnmajor_desc(smem) : sm100::sw128_kmajor_desc(smem)) +
                                  (Smem::kABytes >> 4);
@@ -206,6 +211,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int k_blocks = blocks_of(g);
             if (k_blocks == 0) continue;
             const uint32_t acc = n_acc & 1;
+            const uint32_t idesc =
+                (half_tile(g, mt) ? sm100::idesc_bf16_f32(64, kBN) : sm100::idesc_bf16_f32(kBM, kBN)) | majors;
             ok = sm100::mbar_wait(&tmem_empty[acc], ((n_acc >> 1) & 1) ^ 1);
             const uint32_t d = tmem_base + acc * kBN;
             for (int kb = 0; ok && kb < k_blocks; ++kb, ++it) {
@@ -253,19 +260,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         const int q = warp & 3;
         const int half = warp >> 2;
-        const int row_in_tile = q * 32 + lane;
         T* const out = static_cast<T*>(p.a.out);
         uint8_t* stg = smem + Smem::kStgOffset + warp * kRowStoreBytes;
         uint32_t n_acc = 0;
         for (int tile = blockIdx.x; tile < total_tiles && !aborted(); tile += gridDim.x) {
             int g, mt, nt;
             locate(tile, g, mt, nt);
-            const int64_t row = MODE == kWgrad
-                                    ? static_cast<int64_t>(g) * p.m_cols + mt * kBM + row_in_tile
-                                    : static_cast<int64_t>(table.off[g]) + mt * kBM + row_in_tile;
-            const int64_t r0 = row - lane;  // the warp's first row, and how many of its rows are the result's
+            // The warp's rows: r0 + lane, `rows` of them in the result.
+            const int span = half_tile(g, mt) ? 16 : 32;
+            const int64_t r0 = (MODE == kWgrad ? static_cast<int64_t>(g) * p.m_cols : table.off[g]) + mt * kBM + q * span;
             const int64_t r_end = MODE == kWgrad ? static_cast<int64_t>(g + 1) * p.m_cols : table.off[g + 1];
-            const int rows = static_cast<int>(r_end - r0 < 32 ? r_end - r0 : 32);
+            const int rows = static_cast<int>(r_end - r0 < span ? r_end - r0 : span);
             const int col0 = nt * kBN + half * (kBN / 2);
             const int cols = p.n_cols - col0;  // a multiple of 64
             const bool have = blocks_of(g) != 0;

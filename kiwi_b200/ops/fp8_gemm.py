@@ -32,6 +32,17 @@ from .grouped_gemm import _swiglu_tiles
 
 _BLOCK = 128
 _FP8 = torch.float8_e4m3fn
+_ops = None
+
+
+def _native_ops():
+    """The native extension's ops, looked up once: a call of a few microseconds pays for every lookup."""
+    global _ops
+    if _ops is None:
+        from .. import native
+
+        _ops = native().ops
+    return _ops
 
 
 def _check_operand(x, s, scale_rows, what):
@@ -115,9 +126,7 @@ def fp8_gemm(a, a_scale, b, b_scale, out=None):
         _check(a, a_scale, b, b_scale, None, out, False, None)
         res = fp8_gemm_reference(a, a_scale, b, b_scale).bfloat16()
         return res if out is None else out.copy_(res)
-    from .. import native
-
-    return native().ops.fp8_gemm(a, a_scale, b, b_scale, None, out)
+    return _native_ops().fp8_gemm(a, a_scale, b, b_scale, None, out)
 
 
 def grouped_fp8_gemm(a, a_scale, b, b_scale, counts, out=None, swiglu=False, row_scale=None):
@@ -133,9 +142,7 @@ def grouped_fp8_gemm(a, a_scale, b, b_scale, counts, out=None, swiglu=False, row
             return res
         out[:total] = res[:total]
         return out
-    from .. import native
-
-    return native().ops.fp8_gemm(a, a_scale, b, b_scale, counts, out, bool(swiglu), row_scale)
+    return _native_ops().fp8_gemm(a, a_scale, b, b_scale, counts, out, bool(swiglu), row_scale)
 
 
 def grouped_fp8_swiglu(a, a_scale, b, b_scale, counts):
@@ -148,9 +155,7 @@ def grouped_fp8_swiglu(a, a_scale, b, b_scale, counts):
         _check(a, a_scale, b, b_scale, counts, None, True, None)
         _checked_sum(counts, a.shape[0])
         return _moe.quant_fp8_codes(fp8_gemm_reference(a, a_scale, b, b_scale, counts, True))
-    from .. import native
-
-    return native().ops.fp8_swiglu(a, a_scale, b, b_scale, counts)
+    return _native_ops().fp8_swiglu(a, a_scale, b, b_scale, counts)
 
 
 def expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale=None, out=None):
@@ -165,9 +170,7 @@ def expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale=N
             raise ValueError("w13 must be [E * 2F, H] and w2 [E * H, F]")
         h, hs = grouped_fp8_swiglu(x, x_scale, w13, w13_scale, counts)
         return grouped_fp8_gemm(h, hs, w2, w2_scale, counts, out, False, row_scale)
-    from .. import native
-
-    return native().ops.expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale, out)
+    return _native_ops().expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale, out)
 
 
 def quant_fp8_weights(w):
@@ -185,21 +188,17 @@ def quant_fp8_weights(w):
         codes, scales = _moe.quant_fp8_codes(t, _BLOCK * _BLOCK)
         codes = codes.view(rb, cb, _BLOCK, _BLOCK).permute(0, 2, 1, 3).reshape(rb * _BLOCK, cb * _BLOCK)
         return codes[:r, :c].contiguous(), scales.view(rb, cb)
-    from .. import native
-
-    return native().ops.quant_fp8_weights(w)
+    return _native_ops().quant_fp8_weights(w)
 
 
 def check_gemm(device=None):
     """Raises RuntimeError if a product of this module or of
     :mod:`kiwi_b200.ops.grouped_linear` on ``device`` (the current one) reported
     an error since the last check (synchronises the current stream)."""
-    from .. import native
-
     dev = torch.cuda.current_device() if device is None else torch.device(device).index
     if dev is None:
         dev = torch.cuda.current_device()
-    e = native().ops.gemm_error(dev)
+    e = _native_ops().gemm_error(dev)
     if e:
         what = [n for b, n in ((1, "a wait ran out"), (2, "counts negative or past the rows")) if e & b]
         raise RuntimeError("expert products: " + " and ".join(what))

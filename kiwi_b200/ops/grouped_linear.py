@@ -32,7 +32,7 @@ Gradients are once differentiable.
 """
 import torch
 
-from .fp8_gemm import _as_counts, _checked_sum
+from .fp8_gemm import _as_counts, _checked_sum, _native_ops
 from .grouped_gemm import grouped_gemm_reference
 
 
@@ -78,9 +78,7 @@ def grouped_linear_dgrad(dy, w, counts, out=None):
     """dx [rows, K] of :func:`grouped_linear` for dy [rows, N]."""
     counts = _as_counts(counts, dy.device)
     if dy.is_cuda:
-        from .. import native
-
-        return native().ops.grouped_linear_dgrad(dy, w, counts, out)
+        return _native_ops().grouped_linear_dgrad(dy, w, counts, out)
     _check_counts(counts)
     if w.dtype != torch.bfloat16 or w.dim() != 2 or w.shape[0] != counts.numel() * dy.shape[-1]:
         raise ValueError("w must be bf16 [groups * N, K] with dy's N")
@@ -101,9 +99,7 @@ def grouped_linear_wgrad(dy, x, counts, out=None, accumulate=False):
     fp32); with ``accumulate`` it is added to ``out``."""
     counts = _as_counts(counts, dy.device)
     if dy.is_cuda:
-        from .. import native
-
-        return native().ops.grouped_linear_wgrad(dy, x, counts, out, bool(accumulate))
+        return _native_ops().grouped_linear_wgrad(dy, x, counts, out, bool(accumulate))
     _check_counts(counts)
     if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[0] != dy.shape[0]:
         raise ValueError("x must be bf16 [rows, K] with dy's rows")
@@ -146,9 +142,7 @@ def grouped_linear(x, w, counts, out=None):
         if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
             raise ValueError("out is not differentiable: leave it out, or call under torch.no_grad()")
     if x.is_cuda:
-        from .. import native
-
-        o = native().ops
+        o = _native_ops()
         return o.grouped_linear(x, w, counts) if out is None else o.grouped_linear_out(x, w, counts, out)
     return _GroupedLinear.apply(x, w, counts) if out is None else _forward(x, w, counts, out)
 
@@ -170,9 +164,7 @@ def swiglu_grad(dh, y, row_scale=None, need_scale_grad=None):
     (or with ``need_scale_grad=False``)."""
     need = row_scale is not None if need_scale_grad is None else bool(need_scale_grad)
     if y.is_cuda:
-        from .. import native
-
-        return native().ops.swiglu_grad(dh, y, row_scale, need)
+        return _native_ops().swiglu_grad(dh, y, row_scale, need)
     _check_swiglu(y, row_scale)
     if dh.dtype != torch.bfloat16 or dh.dim() != 2 or tuple(dh.shape) != (y.shape[0], y.shape[1] // 2):
         raise ValueError("dh must be bf16 [rows, F] for y [rows, 2F]")
@@ -207,9 +199,7 @@ def swiglu(y, row_scale=None):
     """bf16 [rows, F] of y [rows, 2F] (blocks of 128 gate and 128 up columns),
     times ``row_scale`` (fp32 [rows]); differentiable in both."""
     if y.is_cuda:
-        from .. import native
-
-        return native().ops.swiglu(y, row_scale)
+        return _native_ops().swiglu(y, row_scale)
     return _SwiGLU.apply(y, row_scale)
 
 

@@ -8,6 +8,11 @@ from kiwi_b200 import ops
 BF16, F32 = 2.0 ** -8, 2.0 ** -23
 
 
+@pytest.fixture(autouse=True)
+def _seed():
+    torch.manual_seed(0)
+
+
 def _fp8(groups, n, k, rows, seed=0):
     g = torch.Generator().manual_seed(seed)
     a = torch.randn(rows, k, generator=g).mul(50).to(torch.float8_e4m3fn)
@@ -124,7 +129,13 @@ def test_weight_gradient_accumulates():
 @pytest.mark.parametrize("rows", [0, 1, 6])
 def test_ffn_gradients_against_autograd(rows):
     """The chain's gradients against autograd of the 64-bit formula: at most three
-    roundings of rows to bf16 and one of the gradient, 2^-8 of a value each."""
+    roundings of rows to bf16 and one of the gradient, 2^-8 of a value each.
+
+    A routing weight's gradient is one sum, sum_j dh_j a_j u_j with a = silu(g),
+    which may cancel, so it is bounded term by term: dh, g and u are each off by
+    2^-8 of a value (|silu'| <= 1.1), hence by 2^-8 sum_j |dh_j| (|a_j u_j| +
+    1.1 |g_j u_j| + |a_j u_j|), and 5 % for products of errors."""
+    torch.manual_seed(rows)
     h, f = 64, 128
     counts = [rows // 2, rows - rows // 2]
     x = torch.randn(rows, h).bfloat16()
@@ -137,15 +148,21 @@ def test_ffn_gradients_against_autograd(rows):
     grads = torch.autograd.grad(out, leaves, d)
     auto = [t.double().requires_grad_() for t in (x, w13, w2, s)]
     outs, off = [], 0
+    slack = torch.zeros(rows, dtype=torch.float64)
     for e, c in enumerate(counts):
         y = auto[0][off:off + c] @ auto[1][e * 2 * f:(e + 1) * 2 * f].T
         gate, up = y[:, :128], y[:, 128:]
-        outs.append((gate * torch.sigmoid(gate) * up * auto[3][off:off + c, None]) @ auto[2][e * h:(e + 1) * h].T)
+        a = gate * torch.sigmoid(gate)
+        outs.append((a * up * auto[3][off:off + c, None]) @ auto[2][e * h:(e + 1) * h].T)
+        dh = d[off:off + c].double() @ auto[2][e * h:(e + 1) * h]
+        slack[off:off + c] = 1.05 * BF16 * (dh.abs() * (2 * (a * up).abs() + 1.1 * (gate * up).abs())).sum(1).detach()
         off += c
     ref = torch.cat(outs)
     assert (out.double() - ref).norm() <= 3 * BF16 * ref.norm()
-    for got, want in zip(grads, torch.autograd.grad(ref, auto, d.double())):
-        assert (got.double() - want).norm() <= 4 * BF16 * want.norm()
+    want = torch.autograd.grad(ref, auto, d.double())
+    for g, r in zip(grads[:3], want[:3]):
+        assert (g.double() - r).norm() <= 4 * BF16 * r.norm()
+    assert bool(((grads[3].double() - want[3]).abs() <= slack).all())
 
 
 def test_grouped_linear_refusals():
