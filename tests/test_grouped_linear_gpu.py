@@ -317,6 +317,42 @@ def test_captured_step_follows_counts_and_data():
     ops.check_gemm()
 
 
+def test_captured_training_step():
+    """Forward and backward of the FFN in one graph, warmed up on the capturing
+    stream; replays follow the counts, the data and the weights."""
+    counts, h, f = [30, 0, 41], 128, 256
+    g = _gen(17)
+    cnt = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    x = torch.randn(80, h, generator=g, device="cuda").bfloat16().requires_grad_()
+    w13 = (torch.randn(3 * 2 * f, h, generator=g, device="cuda") * 0.1).bfloat16().requires_grad_()
+    w2 = (torch.randn(3 * h, f, generator=g, device="cuda") * 0.1).bfloat16().requires_grad_()
+    s = torch.rand(80, generator=g, device="cuda").requires_grad_()
+    d = torch.randn(80, h, generator=g, device="cuda").bfloat16()
+
+    def step():
+        y = ops.expert_ffn(x, w13, w2, cnt, s)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w13, w2, s), d)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        held = step()
+    for c in ([30, 0, 41], [1, 79, 0], [0, 0, 0]):
+        cnt.copy_(torch.tensor(c))
+        with torch.no_grad():
+            x.mul_(0.9), w2.mul_(1.1)
+        gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+    ops.check_gemm()
+
+
 def test_refusals():
     x, w, dy, cnt = _data(_gen(15), [4, 4], 128, 128)
     bad = [
