@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     GroupTable& table = *reinterpret_cast<GroupTable*>(smem + S::kTableOffset);
-    float* s_amax = reinterpret_cast<float*>(smem + S::kAmaxOffset);  // [tile parity][column half][row]
+    float* s_amax = reinterpret_cast<float*>(smem + S::kAmaxOffset);  // [tile parity][column half][thread]
     float2* s_scale = reinterpret_cast<float2*>(smem + S::kScaleOffset);  // [block parity][row]: for each column part
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBarOffset);
     // done: a block's MMAs have run and its scales are in shared memory.  Its
@@ -146,6 +146,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = table.tiles[groups];
 
+    // A tile with at most 64 rows of its group left runs M = 64 MMAs: half the
+    // tensor work, the same sums.  Its row 16 q + i is in TMEM lane 32 q + i.
+    auto half_tile = [&](int g, int mt) { return table.off[g + 1] - table.off[g] - mt * kBM <= 64; };
+
     auto aborted = [&]() { return *reinterpret_cast<volatile int*>(&s_abort) != 0; };
     auto fail = [&]() {
         *reinterpret_cast<volatile int*>(&s_abort) = 1;
@@ -184,13 +188,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (warp == 9) {
             // The whole warp walks the blocks and one elected lane issues, so that
             // descriptors and addresses are warp-uniform.
-            const uint32_t idesc = sm100::idesc_e4m3_f32(kBM, kBN);
             const uint64_t desc0 = sm100::sw128_kmajor_desc(smem);
             const bool issuer = sm100::elect_one();
             uint32_t it = 0;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x) {
+                int g, mt, nt;
+                find_tile(table, groups, n_tiles, tile, g, mt, nt);
+                const uint32_t idesc =
+                    half_tile(g, mt) ? sm100::idesc_e4m3_f32(64, kBN) : sm100::idesc_e4m3_f32(kBM, kBN);
                 for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                     const uint32_t buf = it & 1;
                     ok = sm100::mbar_wait(&full[stage], phase) && sm100::mbar_wait(&drained[buf], ((it >> 1) & 1) ^ 1);
@@ -261,7 +268,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::reg_inc<kDrainRegs>();
         const int q = warp & 3;
         const int half = warp >> 2;
-        const int row_in_tile = q * 32 + lane;
         uint8_t* stg = smem + S::kStgOffset + warp * kRowStoreBytes;
         const bool vec = p.a.ldc % 8 == 0 && reinterpret_cast<uintptr_t>(p.a.c) % 16 == 0;
         uint32_t it = 0;
@@ -271,10 +277,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int tile = blockIdx.x; ok && tile < total_tiles && !aborted(); tile += gridDim.x, ++n_done) {
             int g, mt, nt;
             find_tile(table, groups, n_tiles, tile, g, mt, nt);
-            const int64_t row = static_cast<int64_t>(table.off[g]) + mt * kBM + row_in_tile;
-            const bool valid = row < table.off[g + 1];
-            const int64_t r0 = row - lane;  // the warp's first row, and how many of its rows are the group's
-            const int r_end = static_cast<int>(table.off[g + 1] - r0 < 32 ? table.off[g + 1] - r0 : 32);
+            // The warp's rows: r0 + lane, r_end of them in the group.
+            const int span = half_tile(g, mt) ? 16 : 32;
+            const int row_in_tile = q * span + lane;
+            const int64_t r0 = static_cast<int64_t>(table.off[g]) + mt * kBM + q * span;
+            const int64_t row = r0 + lane;
+            const int r_end = static_cast<int>(table.off[g + 1] - r0 < span ? table.off[g + 1] - r0 : span);
+            const bool valid = lane < r_end;
             uint64_t acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
@@ -355,13 +364,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 64; ++i) amax = fmaxf(amax, fabsf(h[i]));
                     float* slot = s_amax + (n_done & 1) * 2 * kBM;
-                    slot[half * kBM + row_in_tile] = amax;
+                    const int place = q * 32 + lane;  // this thread's own, whatever the tile's height
+                    slot[half * kBM + place] = amax;
                     sm100::mbar_arrive(amax_bar);
                     if (!sm100::mbar_wait(amax_bar, n_done & 1)) {
                         fail();
                         break;
                     }
-                    amax = fmaxf(amax, slot[(half ^ 1) * kBM + row_in_tile]);
+                    amax = fmaxf(amax, slot[(half ^ 1) * kBM + place]);
                     const float scale = amax > 0.f ? amax / ep::kFp8Max : 1.0f;
                     const float inv = amax > 0.f ? ep::kFp8Max / amax : 0.f;
                     uint4 w[4];

@@ -28,9 +28,13 @@ CUtensorMap make_tmap_2d(const void* ptr, CUtensorMapDataType type, int elem, ui
     if (box_cols * elem != 128) throw kiwi::error("make_tmap_2d: box rows must be 128 bytes");
     // A thread that has made no runtime call yet, such as autograd's worker, has
     // no current context, and the driver call below does not bind one.
-    int dev = 0;
-    KIWI_CUDA_CHECK(cudaGetDevice(&dev));
-    KIWI_CUDA_CHECK(cudaSetDevice(dev));
+    static thread_local bool bound = false;
+    if (!bound) {
+        int dev = 0;
+        KIWI_CUDA_CHECK(cudaGetDevice(&dev));
+        KIWI_CUDA_CHECK(cudaSetDevice(dev));
+        bound = true;
+    }
     CUtensorMap m;
     const cuuint64_t dims[2] = {cols, rows};
     const cuuint64_t strides[1] = {ld_bytes};
