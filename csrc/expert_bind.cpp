@@ -124,8 +124,8 @@ Fp8Call fp8_call(const torch::Tensor& a, const torch::Tensor& a_scale, const tor
     return c;
 }
 
-torch::Tensor fp8_gemm_py(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
-                          OptTensor counts, OptTensor out, bool swiglu, OptTensor row_scale) {
+torch::Tensor fp8_gemm_out(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
+                           OptTensor counts, OptTensor out, bool swiglu, OptTensor row_scale, bool follows) {
     require(a.is_cuda(), "A must be a CUDA tensor");
     const c10::cuda::CUDAGuard guard(a.device());
     Fp8Call c = fp8_call(a, a_scale, b, b_scale, counts);
@@ -146,14 +146,21 @@ torch::Tensor fp8_gemm_py(torch::Tensor a, torch::Tensor a_scale, torch::Tensor 
     c.args.row_scale = row_scale ? row_scale->data_ptr<float>() : nullptr;
     c.args.swiglu = swiglu;
     c.args.zero_tail = !out && counts;
+    c.args.follows = follows;
     gemm::fp8_gemm(c.args, cur_stream());
     return o;
+}
+
+torch::Tensor fp8_gemm_py(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
+                          OptTensor counts, OptTensor out, bool swiglu, OptTensor row_scale) {
+    return fp8_gemm_out(a, a_scale, b, b_scale, counts, out, swiglu, row_scale, false);
 }
 
 /// The gate and up product with its SwiGLU rows quantised to FP8.
 std::pair<torch::Tensor, torch::Tensor> fp8_swiglu_quant(const torch::Tensor& a, const torch::Tensor& a_scale,
                                                          const torch::Tensor& b, const torch::Tensor& b_scale,
-                                                         const torch::Tensor& counts, bool zero_tail) {
+                                                         const torch::Tensor& counts, bool zero_tail,
+                                                         bool feeds_next) {
     Fp8Call c = fp8_call(a, a_scale, b, b_scale, counts);
     require(c.args.n % 256 == 0, "SwiGLU needs N to be a multiple of 256");
     torch::Tensor codes = torch::empty({a.size(0), c.args.n / 2}, a.options());
@@ -162,6 +169,7 @@ std::pair<torch::Tensor, torch::Tensor> fp8_swiglu_quant(const torch::Tensor& a,
     c.args.scales = scales.data_ptr<float>();
     c.args.swiglu = true;
     c.args.zero_tail = zero_tail;
+    c.args.feeds_next = feeds_next;
     gemm::fp8_gemm(c.args, cur_stream());
     return {codes, scales};
 }
@@ -170,7 +178,7 @@ py::tuple fp8_swiglu_py(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b,
                         torch::Tensor counts) {
     require(a.is_cuda(), "A must be a CUDA tensor");
     const c10::cuda::CUDAGuard guard(a.device());
-    auto r = fp8_swiglu_quant(a, a_scale, b, b_scale, counts, true);
+    auto r = fp8_swiglu_quant(a, a_scale, b, b_scale, counts, true, false);
     return py::make_tuple(r.first, r.second);
 }
 
@@ -192,8 +200,8 @@ torch::Tensor expert_ffn_fp8_py(torch::Tensor x, torch::Tensor x_scale, torch::T
     check_row_scale(row_scale, x.size(0), x.device());
     require(x.size(1) % 128 == 0, "H must be a multiple of 128");
     check_fp8_operand(w2, w2_scale, w2.size(0) / 128, x.device(), "w2");
-    auto h = fp8_swiglu_quant(x, x_scale, w13, w13_scale, counts, false);
-    return fp8_gemm_py(h.first, h.second, w2, w2_scale, counts, out, false, row_scale);
+    auto h = fp8_swiglu_quant(x, x_scale, w13, w13_scale, counts, false, true);
+    return fp8_gemm_out(h.first, h.second, w2, w2_scale, counts, out, false, row_scale, true);
 }
 
 py::tuple quant_fp8_weights_py(torch::Tensor w) {

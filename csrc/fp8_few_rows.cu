@@ -124,6 +124,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (split > 1) sm100::cluster_sync();  // every CTA's barriers exist before any arrival from another
     sm100::tc_fence_after();
+    if (p.a.feeds_next) sm100::grid_launch_dependents();
+    if (p.a.follows) sm100::grid_wait_before();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = table.tiles[groups];
 
@@ -385,17 +387,8 @@ void launch(const Params& p, const CUtensorMap& tb, int split, cudaStream_t stre
                              ? ((p.a.rows + ROWS - 1) / ROWS + (p.a.num_groups < p.a.rows ? p.a.num_groups : p.a.rows)) * n_tiles
                              : (p.a.rows + ROWS - 1) / ROWS * n_tiles;
     const int64_t workers = num_sms() / split;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim = {static_cast<unsigned>(split), 1, 1};
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(most < workers ? most : workers) * split);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = &cluster;
-    cfg.numAttrs = split > 1 ? 1 : 0;
-    KIWI_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp8_few_rows_kernel<EPI, ROWS>, ta, tb, p, split));
+    launch_kernel(fp8_few_rows_kernel<EPI, ROWS>, static_cast<unsigned>(most < workers ? most : workers) * split, kThreads,
+                  smem, split, p.a.follows, stream, ta, tb, p, split);
 }
 
 template <int EPI>

@@ -143,6 +143,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm100::tc_fence_before();
     __syncthreads();
     sm100::tc_fence_after();
+    if (p.a.feeds_next) sm100::grid_launch_dependents();
+    if (p.a.follows) sm100::grid_wait_before();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = table.tiles[groups];
 
@@ -486,8 +488,8 @@ void launch(const Params& p, cudaStream_t stream) {
     // At most this many tiles, however the rows fall into groups.
     const int64_t most = ((a.rows + kBM - 1) / kBM + (a.counts ? a.num_groups : 0)) * ((a.n + kBN - 1) / kBN);
     const int sms = num_sms();
-    fp8_gemm_kernel<EPI><<<static_cast<unsigned>(most < sms ? most : sms), kThreads, Smem::kBytes, stream>>>(ta, tb, p);
-    KIWI_CUDA_CHECK(cudaGetLastError());
+    launch_kernel(fp8_gemm_kernel<EPI>, static_cast<unsigned>(most < sms ? most : sms), kThreads, Smem::kBytes, 1,
+                  a.follows, stream, ta, tb, p);
 }
 
 struct Choice {

@@ -28,6 +28,30 @@ void launch_few_rows(const Params& p, int row_chunk, int split, cudaStream_t str
 
 #if defined(__CUDACC__)
 
+/// A launch in clusters of `cluster` CTAs that may start before the kernel ahead of it has ended (`follows`).
+template <typename... Formal, typename... Actual>
+void launch_kernel(void (*kernel)(Formal...), unsigned grid, int threads, int smem, int cluster, bool follows,
+                   cudaStream_t stream, const Actual&... args) {
+    cudaLaunchAttribute attr[2] = {};
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n++].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    }
+    if (follows) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    KIWI_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, Formal(args)...));
+}
+
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));

@@ -31,6 +31,13 @@ struct Fp8GemmArgs {
     float* scales;            // ... with [rows, n / 256] scales amax / 448 (1 for an all-zero block)
     const float* row_scale;   // optional [rows]: factor of an output row (bf16 output)
     bool swiglu;              // B holds blocks of 128 gate and 128 up rows; n a multiple of 256
+    // Two products in a row on a stream, the second on the first's output: the
+    // first sets feeds_next, the second follows, and its CTAs then start up while
+    // the last of the first's are still running.  Nothing but the first's output
+    // may be written by it and read by the second, and the first is launched
+    // without `follows`, so that all earlier work is done.
+    bool feeds_next;
+    bool follows;
     bool zero_tail;           // rows past the last group's are set to zero (else left as they were)
 };
 

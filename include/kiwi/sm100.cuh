@@ -297,6 +297,16 @@ KIWI_DEV void tmem_wait_16cols(uint32_t (&r)[16]) {
                  : "memory");
 }
 
+// ---- overlap of a kernel's start with the end of the one before it on the stream ----
+
+/// Lets the next kernel, if it was launched to follow programmatically, start
+/// once every CTA has come here or exited.
+KIWI_DEV void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+/// Waits until the kernel before this one has finished and its writes are
+/// visible (at once in a kernel that was launched as usual).
+KIWI_DEV void grid_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- registers between warpgroups (whole warpgroup; the shares must not exceed the launch's total) ----
 
 template <int N>
