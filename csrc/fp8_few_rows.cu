@@ -17,6 +17,11 @@
 // A group with more than ROWS rows is cut into chunks of ROWS, which read the
 // same weights, mostly from L2.  (Chunks of 64 rows were no faster at any size.)
 //
+// Bound by weight streaming, and for the smallest calls by launch and set-up.
+// Measured on one B200 (graph, warm): 1 row, 7168 x 2048 in 6.9 us; 33 rows,
+// 4096 x 7168 in 13 us; 32 rows for each of 32 experts, 4096 x 7168 (940 MB of
+// weights) in 150 us = 6.3 TB/s.
+//
 //   warps 0..7   drain: TMEM lane quadrant = warp % 4, weight block = warp / 4;
 //                then a token's 256 columns a warp
 //   warp 8       TMA producer      warp 9  TMEM owner and MMA issuer

@@ -25,7 +25,26 @@ inline constexpr uint32_t kGemmCounts = 2u;    // a negative count, or counts wh
 struct GroupTable {
     int32_t off[kMaxGroups + 1];
     int32_t tiles[kMaxGroups + 1];
+    int32_t chunk_tiles[kMaxGroups / 32];  // scratch of the scan: sums of 32 groups
+    int64_t chunk_rows[kMaxGroups / 32];
 };
+
+template <typename T>
+__device__ __forceinline__ T warp_inclusive_scan(T v) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const T y = __shfl_up_sync(0xffffffffu, v, d);
+        if ((threadIdx.x & 31) >= d) v += y;
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T warp_sum(T v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
 
 /// Whole CTA; ends with a __syncthreads().  Counts are clamped to what `rows`
 /// can hold, so every offset is a valid row whatever the counts are (a bad
@@ -53,50 +72,39 @@ __device__ __forceinline__ void build_group_table(GroupTable& t, const int32_t* 
         t.off[g + 1] = c;
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        const int per = (groups + 31) / 32;
-        const int g0 = lane * per;
-        const int g1 = g0 + per < groups ? g0 + per : groups;
-        int64_t sum = 0;
-        for (int g = g0; g < g1; ++g) sum += t.off[g + 1];
-        int64_t incl = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += y;
+    // A warp takes 32 groups at a time: first their rows, then, with the rows
+    // before them known, their offsets and tiles, then the tiles before them.
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (int ch = warp; ch * 32 < groups; ch += warps) {
+        const int g = ch * 32 + lane;
+        const int64_t sum = warp_sum(static_cast<int64_t>(g < groups ? t.off[g + 1] : 0));
+        if (lane == 0) t.chunk_rows[ch] = sum;
+    }
+    __syncthreads();
+    for (int ch = warp; ch * 32 < groups; ch += warps) {
+        const int g = ch * 32 + lane;
+        const int32_t c = g < groups ? t.off[g + 1] : 0;
+        const int64_t before = warp_sum(lane < ch ? t.chunk_rows[lane] : int64_t{0});
+        const int64_t upto = before + warp_inclusive_scan(static_cast<int64_t>(c));
+        const int64_t first = upto - c < rows ? upto - c : rows;
+        const int64_t last = upto < rows ? upto : rows;
+        if (upto > rows) bad = true;
+        const int32_t tl = warp_inclusive_scan(static_cast<int32_t>((last - first + bm - 1) / bm) * n_tiles);
+        if (g < groups) {
+            t.off[g + 1] = static_cast<int32_t>(last);
+            t.tiles[g + 1] = tl;
         }
-        int64_t at = incl - sum;
-        int32_t tl = 0;  // this lane's tiles
-        int64_t pos = at;
-        for (int g = g0; g < g1; ++g) {
-            const int64_t end = pos + t.off[g + 1];
-            const int64_t c = (end < rows ? end : rows) - (pos < rows ? pos : rows);
-            tl += static_cast<int32_t>((c + bm - 1) / bm);
-            pos = end;
-        }
-        int32_t tincl = tl;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int32_t y = __shfl_up_sync(0xffffffffu, tincl, d);
-            if (lane >= d) tincl += y;
-        }
-        int32_t tile = (tincl - tl) * n_tiles;
-        pos = at;
-        for (int g = g0; g < g1; ++g) {
-            const int64_t first = pos < rows ? pos : rows;
-            const int64_t end = pos + t.off[g + 1];
-            const int64_t last = end < rows ? end : rows;
-            if (end > rows) bad = true;
-            tile += static_cast<int32_t>((last - first + bm - 1) / bm) * n_tiles;
-            t.off[g + 1] = static_cast<int32_t>(last);  // this lane alone reads and writes its groups' entries
-            t.tiles[g + 1] = tile;
-            pos = end;
-        }
-        if (lane == 0) {
-            t.off[0] = 0;
-            t.tiles[0] = 0;
-        }
+        if (lane == 31) t.chunk_tiles[ch] = tl;
+    }
+    __syncthreads();
+    for (int ch = warp; ch * 32 < groups; ch += warps) {
+        const int g = ch * 32 + lane;
+        const int32_t before = warp_sum(lane < ch ? t.chunk_tiles[lane] : 0);
+        if (g < groups) t.tiles[g + 1] += before;
+    }
+    if (threadIdx.x == 0) {
+        t.off[0] = 0;
+        t.tiles[0] = 0;
     }
     if (bad && error && blockIdx.x == 0) atomicOr(error, kGemmCounts);
     __syncthreads();
