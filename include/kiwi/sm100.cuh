@@ -370,6 +370,14 @@ KIWI_DEV float4 ld_cluster_f32x4(const void* p, uint32_t rank) {
     return v;
 }
 
+/// Arrive on an mbarrier given by its cluster-window address without a
+/// cluster-scope release (which would wait for this thread's stores): for
+/// signals that hand over TMEM, which the tcgen05 fences around them order, and
+/// no memory.
+KIWI_DEV void mbar_arrive_remote(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 /// 2-SM TMA load into this CTA's shared memory whose transaction bytes complete
 /// on the barrier at cluster address `bar_cluster` (the pair leader's barrier).
 KIWI_DEV void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar_cluster, int32_t x, int32_t y) {
@@ -406,6 +414,15 @@ KIWI_DEV void mma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, u
 KIWI_DEV void mma_commit_pair(uint32_t bar_cluster) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster)
                  : "memory");
+}
+
+/// mma_commit_pair to the barrier at the same offset in both CTAs of the pair, in one instruction.
+KIWI_DEV void mma_commit_both(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
 }
 
 #endif  // __CUDACC__

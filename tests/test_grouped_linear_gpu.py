@@ -46,7 +46,8 @@ def _groups(counts):
 
 
 CASES = [([5], 64, 64), ([0, 0, 130, 1], 128, 192), ([256, 0, 77], 320, 448), ([1] * 9, 64, 320), ([0, 0], 128, 256),
-         ([64, 65, 128, 129, 63], 192, 64), ([1000, 3], 256, 512), ([31, 33, 2], 1024, 128)]
+         ([64, 65, 128, 129, 63], 192, 64), ([1000, 3], 256, 512), ([31, 33, 2], 1024, 128),
+         ([257, 513, 255], 320, 448), ([300, 0, 33, 770, 256, 1], 64, 576), ([2000, 700, 95], 2560, 1024)]
 
 
 @pytest.mark.parametrize("counts,n,k", CASES, ids=str)
