@@ -323,9 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     } else {  // all of the accumulator is in registers: the next MMAs may have it
                         sm100::tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) {
-                            sm100::mbar_arrive(&drained[buf]);
-                        }
+                        if (lane == 0) sm100::mbar_arrive(&drained[buf]);
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -571,11 +569,17 @@ void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream) {
     if (args.num_groups > 1 && args.n % 128 != 0) throw kiwi::error("fp8_gemm: grouped N must be a multiple of 128");
     if (args.swiglu && args.n % kBN != 0) throw kiwi::error("fp8_gemm: SwiGLU needs N to be a multiple of 256");
     if (args.codes && !args.swiglu) throw kiwi::error("fp8_gemm: FP8 output needs swiglu");
+    if (args.codes && (!args.scales || reinterpret_cast<uintptr_t>(args.codes) % 16 != 0)) {
+        throw kiwi::error("fp8_gemm: FP8 output needs codes on a 16-byte boundary and scales");
+    }
     if (args.rows < 0 || args.rows > INT32_MAX - kBM ||
         static_cast<int64_t>(args.num_groups) * args.n > INT32_MAX - kBN) {
         throw kiwi::error("fp8_gemm: more than 2^31 rows");
     }
     if (args.rows == 0) return;
+    if (!args.a || !args.b || !args.a_scale || !args.b_scale || (!args.c && !args.codes)) {
+        throw kiwi::error("fp8_gemm: missing operands or output");
+    }
     Params p{};
     p.a = args;
     p.k_blocks = (args.k + kBK - 1) / kBK;
@@ -591,6 +595,9 @@ void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream) {
 void quant_fp8_blocks(const __nv_bfloat16* w, int64_t ld, int64_t rows, int64_t cols, uint8_t* codes, float* scales,
                       cudaStream_t stream) {
     if (rows <= 0 || cols <= 0) return;
+    if (!w || !codes || !scales || reinterpret_cast<uintptr_t>(codes) % 16 != 0) {
+        throw kiwi::error("quant_fp8_blocks: missing tensors, or codes off a 16-byte boundary");
+    }
     const int64_t cb = (cols + 127) / 128, blocks = (rows + 127) / 128 * cb;
     if (blocks > INT32_MAX) throw kiwi::error("quant_fp8_blocks: matrix too large");
     quant_fp8_blocks_kernel<<<static_cast<unsigned>(blocks), kQuantThreads, 0, stream>>>(

@@ -16,8 +16,10 @@ SwiGLU, whose gate and up rows are interleaved in blocks of 128:
 :func:`kiwi_b200.models.moe.interleave_gate_up`).
 
 CUDA tensors run the sm_100a kernel (``kiwi_b200._C.ops.fp8_gemm``: tcgen05 8-bit
-MMAs, scales applied in fp32) on the current stream; nothing synchronises, the
-row counts stay on the device, and every call can be captured into a CUDA graph.
+MMAs, scales applied in fp32) on the current stream; nothing synchronises, row
+counts that are on the device stay there, and such a call can be captured into a
+CUDA graph.  The kernel is chosen by the call's sizes, so the order of a row's
+fp32 sum, and with it the last bit, can change with the number of rows beside it.
 A result that a call allocates has zeros in the rows past ``sum(counts)``; of an
 ``out`` that is passed in, those rows are left as they were.  Counts that are
 negative or add up to more than the rows are clamped and reported, like a wait
@@ -83,9 +85,13 @@ def _check(a, a_scale, b, b_scale, counts, out, swiglu, row_scale):
 
 
 def _as_counts(counts, device):
+    """int32 row counts on the rows' device (a host list is copied there)."""
     if torch.is_tensor(counts) and counts.dtype == torch.int32 and counts.device == device:
         return counts
-    return torch.as_tensor(counts).to(device=device, dtype=torch.int32)
+    counts = torch.as_tensor(counts)
+    if counts.is_floating_point() and counts.numel():
+        raise ValueError("counts must be whole numbers")
+    return counts.to(device=device, dtype=torch.int32)
 
 
 def dequant_fp8(codes, scales, rows_per_scale=1):

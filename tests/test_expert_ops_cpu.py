@@ -85,6 +85,7 @@ def test_fp8_refusals():
         lambda: ops.grouped_fp8_gemm(a, sa, b, sb, cnt, row_scale=torch.ones(7)),
         lambda: ops.grouped_fp8_gemm(a, sa, b, sb, torch.tensor([5, 4])),
         lambda: ops.grouped_fp8_gemm(a, sa, b, sb, torch.tensor([-1, 4])),
+        lambda: ops.grouped_fp8_gemm(a, sa, b, sb, [1.5, 2.0]),
         lambda: ops.grouped_fp8_gemm(a, sa, b, sb, torch.zeros(0, dtype=torch.int32)),
         lambda: ops.expert_ffn_fp8(a, sa, b, sb, b, sb, cnt),
         lambda: ops.quant_fp8_weights(a),

@@ -326,6 +326,7 @@ def test_refusals():
         lambda: ops.grouped_fp8_gemm(a, sa, b[:256], sb[:2], cnt, swiglu=True),
         lambda: ops.grouped_fp8_gemm(a, sa, b, sb, cnt, row_scale=torch.ones(7, device="cuda")),
         lambda: ops.grouped_fp8_gemm(a, sa, b, sb, torch.zeros(0, dtype=torch.int32, device="cuda")),
+        lambda: ops.grouped_fp8_gemm(a, sa, b, sb, [1.5, 2.0]),
         lambda: ops.expert_ffn_fp8(a, sa, b, sb, b, sb, cnt),
         lambda: ops.quant_fp8_weights(a),
     ]
