@@ -17,10 +17,10 @@
 // and its drain 256 FP32-pipe cycles, but an accumulator's round trip (MMAs ~720
 // cycles from issue to completion, drain, hand-over) makes a block ~820 cycles
 // on an idle GPU; in long runs the power cap holds the clock at 1.4 to 1.6 GHz.
-// Measured on one B200: 4096 x 4096 x 7168 in 121 us (1.99 PFLOP/s, 1.19 of the
+// Measured on one B200: 4096 x 4096 x 7168 in 117 us (2.05 PFLOP/s, 1.23 of the
 // measured bf16 rate); gate and up product with SwiGLU and quantisation of
-// 32768 rows over 32 experts (4096 x 7168) in 1011 us (1.90 PFLOP/s), the down
-// product (7168 x 2048) in 585 us (1.64).  Four accumulators of 128 columns,
+// 32768 rows over 32 experts (4096 x 7168) in 982 us (1.96 PFLOP/s), the down
+// product (7168 x 2048) in 570 us (1.69).  Four accumulators of 128 columns,
 // with twice the hand-overs, took 15 to 25 % longer; pairs of SMs sharing a tile
 // took as long at the largest sizes and longer at others.
 //
@@ -64,9 +64,17 @@ constexpr int kThreads = 384;  // two drain warpgroups; one with the producer, t
 constexpr int kDrainThreads = 256;
 constexpr int kScaleWarps = 2;
 // 128 sums and a 32-column TMEM load do not fit the 168 registers that 384
-// threads share evenly; the third warpgroup gives some of its own away.
-constexpr int kDrainRegs = 208, kIssueRegs = 88;
-static_assert(2 * kDrainRegs + kIssueRegs <= 3 * 168, "more registers than the CTA is launched with");
+// threads share evenly; the third warpgroup gives some of its own away.  How many
+// the drain gets is what was fastest without spills; its loop is unrolled, which
+// frees it of moves between the blocks' registers: 4096 x 4096 x 7168 in 117 us
+// against 127, 32768 rows over 32 experts 982 + 570 against 1019 + 598.
+template <int EPI>
+struct Tuning {
+    static constexpr int kDrainRegs = EPI == kEpiStore ? 192 : 208;
+    static constexpr int kIssueRegs = EPI == kEpiStore ? 120 : 88;
+    static constexpr int kUnroll = 4;
+    static_assert(2 * kDrainRegs + kIssueRegs <= 3 * 168, "more registers than the CTA is launched with");
+};
 
 struct Smem {
     static constexpr int kStages = 4;
@@ -168,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp >= 8) {
-        sm100::reg_dec<kIssueRegs>();
+        sm100::reg_dec<Tuning<EPI>::kIssueRegs>();
         if (warp == 8 && lane == 0) {
             uint32_t issued = 0;
             bool ok = true;
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        sm100::reg_inc<kDrainRegs>();
+        sm100::reg_inc<Tuning<EPI>::kDrainRegs>();
         const int q = warp & 3;
         const int half = warp >> 2;
         uint8_t* stg = smem + S::kStgOffset + warp * kRowStoreBytes;
@@ -298,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint64_t acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
-#pragma unroll 1
+#pragma unroll Tuning<EPI>::kUnroll
             for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                 const uint32_t buf = it & 1;
                 if (!sm100::mbar_wait(&done[stage], phase)) {
