@@ -254,6 +254,45 @@ def test_captured_calls_follow_the_counts_and_share_nothing():
     ops.check_gemm()
 
 
+@pytest.mark.parametrize("rows,groups,h,f", [(9, 4, 256, 128), (70, 3, 1024, 512), (3000, 4, 512, 384)])
+def test_captured_ffn_and_calls_in_a_row(rows, groups, h, f):
+    """The FFN's second product starts while its first one ends: in graphs, with
+    other rows and counts from replay to replay, and with calls back to back that
+    reuse each other's memory, each result is that of a call by itself."""
+    g = _gen(rows)
+    x, sx = _rows(g, rows, h)
+    w13, s13 = _weights(g, groups, 2 * f, h)
+    w2, s2 = _weights(g, groups, h, f)
+    scale = torch.rand(rows, generator=g, device="cuda")
+    cnt = torch.zeros(groups, dtype=torch.int32, device="cuda")
+    inputs = []
+    for i in range(3):
+        c = torch.bincount(torch.randint(0, groups, (rows - i,), generator=g, device="cuda"), minlength=groups)
+        inputs.append((_rows(g, rows, h), c.int()))
+    alone = []
+    for (a, sa), c in inputs:
+        hc, hs = ops.grouped_fp8_swiglu(a, sa, w13, s13, c)
+        torch.cuda.synchronize()
+        alone.append(ops.grouped_fp8_gemm(hc, hs, w2, s2, c, row_scale=scale))
+        torch.cuda.synchronize()
+        del hc, hs
+    for _ in range(5):
+        got = [ops.expert_ffn_fp8(a, sa, w13, s13, w2, s2, c, row_scale=scale) for (a, sa), c in inputs]
+        for y, want in zip(got, alone):
+            assert torch.equal(y, want)
+        del got, y
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        one = ops.expert_ffn_fp8(x, sx, w13, s13, w2, s2, cnt, row_scale=scale)
+        two = ops.expert_ffn_fp8(x, sx, w13, s13, w2, s2, cnt, row_scale=scale)
+    for ((a, sa), c), want in zip(inputs, alone):
+        x.view(torch.uint8).copy_(a.view(torch.uint8)), sx.copy_(sa), cnt.copy_(c)
+        for _ in range(3):
+            gr.replay()
+        assert torch.equal(one, want) and torch.equal(two, want)
+    ops.check_gemm()
+
+
 def test_runs_on_the_current_stream():
     g = _gen(8)
     a, sa = _rows(g, 64, 256)
