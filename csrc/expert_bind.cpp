@@ -70,6 +70,13 @@ void check_out(const torch::Tensor& out, int64_t rows, int64_t cols, torch::Scal
                 out.size(1) == cols && (cols == 1 || out.stride(1) == 1) && (rows == 1 || out.stride(0) >= cols),
             "out must be [" + std::to_string(rows) + ", " + std::to_string(cols) + "] with unit column stride, of the "
             "result's type, on the rows' device");
+    require(!out.requires_grad() || !torch::GradMode::is_enabled(),
+            "out requires a gradient: it can only be written under torch.no_grad()");
+}
+
+/// `out` was written: what saved it for a backward pass must find that out.
+void written(const torch::Tensor& out) {
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
 }
 
 /// Whether two tensors' storage ranges meet (an output must not be an input).
@@ -148,6 +155,7 @@ torch::Tensor fp8_gemm_out(torch::Tensor a, torch::Tensor a_scale, torch::Tensor
     c.args.zero_tail = !out && counts;
     c.args.follows = follows;
     gemm::fp8_gemm(c.args, cur_stream());
+    if (out) written(o);
     return o;
 }
 
@@ -267,6 +275,7 @@ torch::Tensor linear_forward_py(torch::Tensor x, torch::Tensor w, torch::Tensor 
     a.ldo = row_stride(o);
     a.zero_tail = !out;
     gemm::grouped_linear_forward(a, cur_stream());
+    if (out) written(o);
     return o;
 }
 
@@ -286,6 +295,7 @@ torch::Tensor linear_dgrad_py(torch::Tensor dy, torch::Tensor w, torch::Tensor c
     a.ldo = row_stride(o);
     a.zero_tail = !out;
     gemm::grouped_linear_dgrad(a, cur_stream());
+    if (out) written(o);
     return o;
 }
 
@@ -310,6 +320,7 @@ torch::Tensor linear_wgrad_py(torch::Tensor dy, torch::Tensor x, torch::Tensor c
     a.out_fp32 = type == torch::kFloat32;
     a.accumulate = accumulate;
     gemm::grouped_linear_wgrad(a, cur_stream());
+    if (out) written(o);
     return o;
 }
 

@@ -112,6 +112,22 @@ def test_rows_behind_the_last_group_of_an_out_are_left():
     assert torch.equal(dx[:30], ops.grouped_linear_dgrad(dy, w, cnt)[:30]) and bool((dx[30:] == 5).all())
 
 
+def test_writing_an_out_is_seen_by_autograd():
+    x, w, dy, cnt = _data(_gen(18), [8, 8], 64, 64)
+    buf = torch.zeros(16, 64, device="cuda", dtype=torch.bfloat16)
+    scale = torch.ones((), device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    z = buf * scale  # saves buf
+    ops.grouped_linear(x, w, cnt, out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    held = torch.zeros(128, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError):
+        ops.grouped_linear_wgrad(dy, x, cnt, out=held)
+    with torch.no_grad():
+        ops.grouped_linear_wgrad(dy, x, cnt, out=held)
+    assert torch.equal(held, ops.grouped_linear_wgrad(dy, x, cnt))
+
+
 def test_no_rows_at_all():
     w = torch.ones(128, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
     x = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
