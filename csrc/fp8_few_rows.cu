@@ -248,6 +248,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step, ++n_sum) {
             int g, mt, nt;
             find_tile(table, groups, n_tiles, tile, g, mt, nt);
+            const int64_t row0 = static_cast<int64_t>(table.off[g]) + mt * ROWS;
+            const int left = table.off[g + 1] - static_cast<int>(row0);
+            const int here = left < ROWS ? left : ROWS;  // tokens of this tile
+            // Lane t holds token t's factor, loaded now and used after the last block.
+            const float factor = EPI != kEpiSwiGLUQuant && p.a.row_scale && lane < here ? __ldg(p.a.row_scale + row0 + lane) : 1.0f;
             uint64_t acc[ROWS / 2];
 #pragma unroll
             for (int i = 0; i < ROWS / 2; ++i) acc[i] = 0;
@@ -282,9 +287,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 next(slot, phase);
             }
             if (!ok) break;
-            const int64_t row0 = static_cast<int64_t>(table.off[g]) + mt * ROWS;
-            const int left = table.off[g + 1] - static_cast<int>(row0);
-            const int here = left < ROWS ? left : ROWS;  // tokens of this tile
             // Every CTA has read the sums of the tile before this one.
             if (n_sum > 0 && !sm100::mbar_wait_cluster(read, (n_sum - 1) & 1)) {
                 fail();
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             for (int t = warp * split + rank; t < here; t += 8 * split) {
                 const int64_t row = row0 + t;
-                const float scale = p.a.row_scale ? __ldg(p.a.row_scale + row) : 1.0f;
+                const float scale = __shfl_sync(0xffffffffu, factor, t);
                 if constexpr (EPI == kEpiStore) {
                     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // columns 8 * lane ..
                     for (int r = 0; r < split; ++r) add8(s_sum + t * kBN + 8 * lane, r, split, f);
