@@ -2,7 +2,7 @@
 //
 // The same sums as csrc/fp8_gemm.cu with the operands' places swapped: 256 rows
 // of the weights are the tensor core's M operand (two of 128: with SwiGLU one
-// of gate and one of up), and up to ROWS rows of the group its N operand.  What
+// of gate and one of up), and up to ROWS (16, 32 or 48) rows of the group its N operand.  What
 // counts here is reading the weights once at the memory's rate: a stage holds
 // 32 KB of weights and only ROWS * 128 bytes of rows, an accumulator 2 * ROWS
 // TMEM columns, so that five of them are in flight and the drain (one FMA per
@@ -15,7 +15,8 @@
 // atomics: the result does not depend on the order of execution.
 //
 // A group with more than ROWS rows is cut into chunks of ROWS, which read the
-// same weights, mostly from L2.  (Chunks of 64 rows were no faster at any size.)
+// same weights, mostly from L2.  (With 64 rows only three
+// stages fit; that was faster at no size.)
 //
 // Bound by weight streaming, and for the smallest calls by launch and set-up.
 // Measured on one B200 (graph, warm): 1 row, 7168 x 2048 in 6.9 us; 33 rows,
@@ -48,11 +49,12 @@ namespace {
 
 constexpr int kThreads = 352;
 constexpr int kDrainThreads = 256;
-// Stages, and TMEM accumulators: the most that fit (4 read weights 4 % slower).
-constexpr int kRing = 5;
 
 template <int ROWS>
 struct Smem {
+    // Stages, and TMEM accumulators: the most that fit (with 32 rows, 4 read weights 4 % slower than 5).
+    static constexpr int kRing = ROWS <= 32 ? 5 : 4;
+    static constexpr int kTmemCols = kRing * 2 * ROWS <= 256 ? 256 : 512;
     static constexpr int kWBytes = kBN * kBK;
     static constexpr int kStageBytes = kWBytes + ROWS * kBK;
     static constexpr int kSumOffset = kRing * kStageBytes;
@@ -61,7 +63,7 @@ struct Smem {
     static constexpr int kBarOffset = kScaleOffset + kRing * 2 * ROWS * 4;
     static constexpr int kBytes = kBarOffset + 256 + 1024;  // barriers, TMEM slot, alignment slack
 };
-static_assert(Smem<32>::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
+static_assert(Smem<32>::kBytes <= 227 * 1024 && Smem<48>::kBytes <= 227 * 1024, "exceeds the shared-memory limit");
 
 /// f += CTA `rank`'s four sums at the place of `p`.
 __device__ __forceinline__ void add4(const float* p, int rank, int split, float* f) {
@@ -82,6 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fp8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                         const __grid_constant__ Params p, const int split) {
     using S = Smem<ROWS>;
+    constexpr int kRing = S::kRing;
     constexpr int kCols = 2 * ROWS;  // TMEM columns of an accumulator
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm100::tma_prefetch_desc(&tmap_a);
         sm100::tma_prefetch_desc(&tmap_b);
     }
-    if (warp == 9) sm100::tmem_alloc(tmem_slot, 8 * kCols);
+    if (warp == 9) sm100::tmem_alloc(tmem_slot, S::kTmemCols);
     build_group_table(table, p.a.counts, groups, p.a.rows, ROWS, n_tiles, p.error);
     sm100::tc_fence_before();
     __syncthreads();
@@ -212,16 +215,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
             int g, mt, nt;
             find_tile(table, groups, n_tiles, tile, g, mt, nt);
+            // A lane a token, and with 48 the first 16 lanes another.
             const int64_t row = static_cast<int64_t>(table.off[g]) + mt * ROWS + lane;
             const int64_t last = table.off[g + 1] - 1;  // rows past the group's are not stored: any scale will do
-            const float* sa = p.a.a_scale + (row < last ? row : last) * p.a.a_scale_stride;
+            const float* sa0 = p.a.a_scale + (row < last ? row : last) * p.a.a_scale_stride;
+            const float* sa1 = p.a.a_scale + (row + 32 < last ? row + 32 : last) * p.a.a_scale_stride;
             const float* sb0 = p.a.b_scale + (static_cast<int64_t>(g) * p.nb + 2 * nt) * p.k_blocks;
             const float* sb1 = 2 * nt + 1 < p.nb ? sb0 + p.k_blocks : sb0;
-            float a = __ldg(sa + kb0), b0 = __ldg(sb0 + kb0), b1 = __ldg(sb1 + kb0);
+            float a0 = __ldg(sa0 + kb0), a1 = ROWS > 32 ? __ldg(sa1 + kb0) : 0.f;
+            float b0 = __ldg(sb0 + kb0), b1 = __ldg(sb1 + kb0);
             for (int kb = kb0; kb < kb1; ++kb) {
-                const float v0 = a * b0, v1 = a * b1;
+                const float v00 = a0 * b0, v01 = a0 * b1, v10 = a1 * b0, v11 = a1 * b1;
                 if (kb + 1 < kb1) {
-                    a = __ldg(sa + kb + 1);
+                    a0 = __ldg(sa0 + kb + 1);
+                    if (ROWS > 32) a1 = __ldg(sa1 + kb + 1);
                     b0 = __ldg(sb0 + kb + 1);
                     b1 = __ldg(sb1 + kb + 1);
                 }
@@ -230,9 +237,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ok = false;
                     break;
                 }
-                if (lane < ROWS) {  // a lane a token
-                    s_scale[(slot * 2 + 0) * ROWS + lane] = v0;
-                    s_scale[(slot * 2 + 1) * ROWS + lane] = v1;
+                float* to = s_scale + slot * 2 * ROWS + lane;
+                if (lane < ROWS) {
+                    to[0] = v00;
+                    to[ROWS] = v01;
+                }
+                if (ROWS > 32 && lane + 32 < ROWS) {
+                    to[32] = v10;
+                    to[ROWS + 32] = v11;
                 }
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&done[slot]);
@@ -251,8 +263,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t row0 = static_cast<int64_t>(table.off[g]) + mt * ROWS;
             const int left = table.off[g + 1] - static_cast<int>(row0);
             const int here = left < ROWS ? left : ROWS;  // tokens of this tile
-            // Lane t holds token t's factor, loaded now and used after the last block.
-            const float factor = EPI != kEpiSwiGLUQuant && p.a.row_scale && lane < here ? __ldg(p.a.row_scale + row0 + lane) : 1.0f;
+            // Lane t holds token t's factor (and token t + 32's), loaded now and used after the last block.
+            const bool scaled = EPI != kEpiSwiGLUQuant && p.a.row_scale;
+            const float factor0 = scaled && lane < here ? __ldg(p.a.row_scale + row0 + lane) : 1.0f;
+            const float factor1 = ROWS > 32 && scaled && lane + 32 < here ? __ldg(p.a.row_scale + row0 + lane + 32) : 1.0f;
             uint64_t acc[ROWS / 2];
 #pragma unroll
             for (int i = 0; i < ROWS / 2; ++i) acc[i] = 0;
@@ -264,16 +278,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 sm100::tc_fence_after();
-                uint32_t v[ROWS];
                 const uint32_t taddr =
                     tmem_base + (static_cast<uint32_t>(q * 32) << 16) + slot * kCols + static_cast<uint32_t>(mb * ROWS);
-                if constexpr (ROWS == 32) {
-                    sm100::tmem_issue_32cols(taddr, v);
-                    sm100::tmem_wait_32cols(v);
-                } else {
-                    sm100::tmem_issue_16cols(taddr, v);
-                    sm100::tmem_wait_16cols(v);
+                uint32_t v[ROWS];
+                if constexpr (ROWS >= 32) sm100::tmem_issue_32cols(taddr, reinterpret_cast<uint32_t(&)[32]>(v));
+                if constexpr (ROWS % 32 != 0) {
+                    sm100::tmem_issue_16cols(taddr + ROWS / 32 * 32, reinterpret_cast<uint32_t(&)[16]>(v[ROWS / 32 * 32]));
+                    sm100::tmem_wait_16cols(reinterpret_cast<uint32_t(&)[16]>(v[ROWS / 32 * 32]));
                 }
+                if constexpr (ROWS >= 32) sm100::tmem_wait_32cols(reinterpret_cast<uint32_t(&)[32]>(v));
                 const float* sc = s_scale + (slot * 2 + mb) * ROWS;
 #pragma unroll
                 for (int i = 0; i < ROWS / 4; ++i) {
@@ -315,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             for (int t = warp * split + rank; t < here; t += 8 * split) {
                 const int64_t row = row0 + t;
-                const float scale = __shfl_sync(0xffffffffu, factor, t);
+                const float scale = __shfl_sync(0xffffffffu, ROWS <= 32 || t < 32 ? factor0 : factor1, t & 31);
                 if constexpr (EPI == kEpiStore) {
                     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // columns 8 * lane ..
                     for (int r = 0; r < split; ++r) add8(s_sum + t * kBN + 8 * lane, r, split, f);
@@ -378,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (split > 1) sm100::cluster_sync();  // no CTA leaves while another may read its sums
     sm100::tc_fence_after();
-    if (warp == 9) sm100::tmem_dealloc(tmem_base, 8 * kCols);
+    if (warp == 9) sm100::tmem_dealloc(tmem_base, S::kTmemCols);
 }
 
 template <int EPI, int ROWS>
@@ -401,7 +414,8 @@ void launch(const Params& p, const CUtensorMap& tb, int split, cudaStream_t stre
 template <int EPI>
 void launch_rows(const Params& p, const CUtensorMap& tb, int rows, int split, cudaStream_t stream) {
     if (rows <= 16) launch<EPI, 16>(p, tb, split, stream);
-    else launch<EPI, 32>(p, tb, split, stream);
+    else if (rows <= 32) launch<EPI, 32>(p, tb, split, stream);
+    else launch<EPI, 48>(p, tb, split, stream);
 }
 
 }  // namespace

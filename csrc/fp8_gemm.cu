@@ -510,23 +510,26 @@ void launch(const Params& p, cudaStream_t stream) {
 }
 
 struct Choice {
-    int row_chunk;  // 0: this file's kernel, else the few-rows kernel with 16 or 32 rows a tile
+    int row_chunk;  // 0: this file's kernel, else the few-rows kernel with 16, 32 or 48 rows a tile
     int split;      // and its CTAs a tile
 };
 
 /// The kernel for a call, by a model of its time in microseconds that was fitted
 /// to a sweep of 1 to 2000 rows (dense N x K 512 x 1024 to 7168 x 2048 and 4096 x
-/// 7168; 16 and 32 experts).  A CTA needs 0.42 us a block of K here, and 0.28 or
-/// 0.32 us with 16 or 32 rows a tile, plus 2.5 or 1.2 us a tile for its start
-/// and epilogue.  Where a tile's K is split, the exchange of its sums costs
-/// another 1.3 us, and several times that on a cluster's second tile, so a split
-/// is only for tiles that the GPU runs all at once; clusters of 4 leave some SMs
-/// of a GPC unused, and how rows fall into experts is not known here (every
-/// expert is taken to end with half a tile), hence the margins.  (Splits of 8
-/// lost to splits of 4.)  No kernel is faster than the weights can be read, at
-/// 6.4 TB/s.  Measured, this file's kernel against few rows: 1 row, 4096 x 7168:
-/// 28.7 / 10.1 us; 64 rows: 29.2 / 13.4; 200: 29.9 / 24.4; 400: 30.6 / 44.1; 32
-/// experts of 32 rows, 4096 x 7168: 171 / 154; of 64 rows: 176 / 200.
+/// 7168; 16 and 32 experts).  A CTA needs 0.37 us a block of K here, and 0.285,
+/// 0.315 or 0.33 us with 16, 32 or 48 rows a tile, plus 2.5 or 1.6 us a tile for
+/// its start and epilogue.  Where a tile's K is split, the exchange of its sums
+/// costs another 1.7 us, and several times that on a cluster's second tile, so a
+/// split is only for tiles that the GPU runs all at once; clusters of 4 leave
+/// some SMs of a GPC unused, and how rows fall into experts is not known here
+/// (every expert is taken to end with half a tile), hence the margins.  (Splits
+/// of 8 lost to splits of 4.)  No kernel is faster than the weights can be read,
+/// at 6.4 TB/s; of kernels that this bounds, few rows are taken (they read with
+/// more in flight) unless their own work is clearly more, and of their tiles the
+/// smaller unless the larger mean clearly less.  Measured, this file's kernel against few
+/// rows: 1 row, 4096 x 7168: 25.7 / 10.1 us; 64 rows: 26.1 / 13.4; 200: 27.9 /
+/// 24.4; 400: 28.6 / 26.4 (48 a tile) or 43.7 (32); 1000: 30.4 / 69; 32 experts of
+/// 32 rows, 4096 x 7168: 162 / 149; of 64 rows: 169 / 199.
 Choice choose(const Fp8GemmArgs& a, int k_blocks) {
     const double sms = num_sms(), n_tiles = (a.n + kBN - 1) / kBN;
     const double used = a.counts ? static_cast<double>(a.rows < a.num_groups ? a.rows : a.num_groups) : 1.0;
@@ -536,15 +539,15 @@ Choice choose(const Fp8GemmArgs& a, int k_blocks) {
         return std::max(used, a.rows / bm + used / 2) * n_tiles;
     };
     Choice best{0, 1};
-    double work = std::ceil(tiles(kBM) / sms) * (0.42 * k_blocks + 2.5), time = std::max(work, hbm);
-    for (int rows : {16, 32}) {
-        const double t = tiles(rows), block = rows == 16 ? 0.28 : 0.32;
+    double work = std::ceil(tiles(kBM) / sms) * (0.37 * k_blocks + 2.5), time = std::max(work, hbm);
+    for (int rows : {16, 32, 48}) {
+        const double t = tiles(rows), block = rows == 16 ? 0.285 : rows == 32 ? 0.315 : 0.33;
         for (int split : {1, 2, 4}) {
             if (split > 1 && (t * split > (a.counts ? 0.6 : 0.87) * sms || split > k_blocks)) break;
-            const double w = split > 1 ? std::ceil(k_blocks / static_cast<double>(split)) * block + 2.5
-                                       : std::ceil(t / sms) * (block * k_blocks + 1.2);
+            const double w = split > 1 ? std::ceil(k_blocks / static_cast<double>(split)) * block + 3.3
+                                       : std::ceil(t / sms) * (block * k_blocks + 1.6);
             const double us = std::max(w, hbm);
-            if (us < time || (us == time && (best.row_chunk == 0 || w < work))) {
+            if (us < time || (us == time && w < (best.row_chunk == 0 ? 1.3 : 0.8) * work)) {
                 best = {rows, split};
                 work = w;
                 time = us;

@@ -53,7 +53,8 @@ def _close(got, ref, slack):
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 256, 128), (2, 7, 144), (33, 129, 112), (64, 1000, 256),
                                    (65, 384, 2064), (127, 255, 640), (129, 257, 384), (300, 640, 1040),
                                    (1, 4096, 2048), (16, 1152, 7168), (700, 2048, 272),
-                                   (2000, 300, 272), (1500, 1003, 528), (3000, 512, 128), (200, 1111, 2064)])
+                                   (2000, 300, 272), (1500, 1003, 528), (3000, 512, 128), (200, 1111, 2064), (400, 4096, 512), (48, 2048, 256),
+                                   (1000, 1111, 272)])
 def test_dense_matches_64_bits(m, n, k):
     g = _gen(m * 7 + n)
     a, sa = _rows(g, m, k)
@@ -65,7 +66,7 @@ def test_dense_matches_64_bits(m, n, k):
     assert torch.equal(out, ops.fp8_gemm(a, sa, b, sb))  # nothing depends on the order of execution
 
 
-COUNTS = [[5], [0, 0, 130, 1], [256, 0, 77], [1] * 9, [0, 0], [64, 65, 128, 129], [1000, 3], [2000, 0, 1, 7000, 130]]
+COUNTS = [[5], [0, 0, 130, 1], [256, 0, 77], [1] * 9, [0, 0], [64, 65, 128, 129], [1000, 3], [2000, 0, 1, 7000, 130], [48, 47, 96, 49] * 7]
 
 
 @pytest.mark.parametrize("counts", COUNTS, ids=str)
