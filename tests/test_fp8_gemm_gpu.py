@@ -46,7 +46,7 @@ def _product(a, sa, b, sb):
 
 
 def _close(got, ref, slack):
-    bad = (got.double() - ref).abs() > BF16 * ref.abs() + slack
+    bad = ~((got.double() - ref).abs() <= BF16 * ref.abs() + slack)  # a NaN is bad
     assert not bool(bad.any()), (int(bad.sum()), got.double()[bad][:4], ref[bad][:4])
 
 
@@ -344,6 +344,33 @@ def test_offsets_past_32_bits():
     assert out.numel() > 2 ** 31
     for r in (slice(0, 3), slice(32767, 32770), slice(m - 3, m)):
         _close(out[r], *_product(a[r], sa[r], b, sb))
+
+
+def _codes(g, rows, k):
+    """Random finite codes, made in place of a conversion's fp32 operand."""
+    c = torch.randint(0, 100, (rows, k), generator=g, device="cuda", dtype=torch.uint8)
+    return c.bitwise_or_(torch.randint(0, 2, (1, k), generator=g, device="cuda", dtype=torch.uint8) << 7).view(torch.float8_e4m3fn)
+
+
+def test_operands_past_32_bits():
+    """Rows of more than 2^31 bytes, and weights of more, of which the last group alone has rows."""
+    m, n, k = 300_001, 16, 7168
+    g = _gen(22)
+    a = _codes(g, m, k)
+    sa = torch.rand(m, k // 128, generator=g, device="cuda")
+    b, sb = _weights(g, 1, n, k)
+    out = ops.fp8_gemm(a, sa, b, sb)
+    for r in (slice(0, 2), slice(299_592, 299_596), slice(m - 2, m)):
+        _close(out[r], *_product(a[r], sa[r], b, sb))
+    groups, n = 33, 9216
+    w = _codes(g, groups * n, k)
+    sw = torch.rand(groups * n // 128, k // 128, generator=g, device="cuda") * 1e-3
+    cnt = torch.zeros(groups, dtype=torch.int32, device="cuda")
+    for rows in (3, 600):
+        cnt[-1] = rows
+        out = ops.grouped_fp8_gemm(a[:rows], sa[:rows], w, sw, cnt)
+        _close(out, *_product(a[:rows], sa[:rows], w[-n:], sw[-n // 128:]))
+    ops.check_gemm()
 
 
 def test_refusals():

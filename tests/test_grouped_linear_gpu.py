@@ -34,7 +34,7 @@ def _close(got, a, b, extra=None, rounding=BF16):
     ref, mag = a @ b, a.abs() @ b.abs()
     if extra is not None:
         ref, mag = ref + extra.double(), mag + extra.double().abs()
-    bad = (got.double() - ref).abs() > rounding * ref.abs() + F32 * (a.shape[1] + 1) * mag
+    bad = ~((got.double() - ref).abs() <= rounding * ref.abs() + F32 * (a.shape[1] + 1) * mag)  # a NaN is bad
     assert not bool(bad.any()), (int(bad.sum()), got.double()[bad][:4], ref[bad][:4])
 
 
@@ -192,6 +192,24 @@ def test_offsets_past_32_bits():
     _close(dx[-2:], y[-2:], w)
 
 
+def test_runs_on_the_current_stream_behind_its_inputs():
+    counts, n, k = [33, 50], 128, 192
+    x, w, dy, cnt = _data(_gen(19), counts, n, k)
+    want = ops.grouped_linear(x, w, cnt), ops.grouped_linear_dgrad(dy, w, cnt), ops.grouped_linear_wgrad(dy, x, cnt)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    late = [torch.zeros_like(t) for t in (x, w, dy, cnt)]
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(2_000_000)
+        for t, v in zip(late, (x, w, dy, cnt)):
+            t.copy_(v)
+        x2, w2, dy2, c2 = late
+        got = ops.grouped_linear(x2, w2, c2), ops.grouped_linear_dgrad(dy2, w2, c2), ops.grouped_linear_wgrad(dy2, x2, c2)
+    s.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 # ---------------------------------------------------------------- SwiGLU
 
 
@@ -234,6 +252,20 @@ def test_swiglu_and_gradients_match_64_bits(rows, ffn, scaled):
     if scaled:
         t = d * gate * sig * up
         assert bool(((grads[1].double() - t.sum(1)).abs() <= ((steps + ffn * F32) * t.abs() + tiny / sc).sum(1)).all())
+
+
+def test_swiglu_offsets_past_32_bits():
+    rows, ffn = 550_000, 2048
+    y = torch.full((rows, 2 * ffn), 0.5, device="cuda", dtype=torch.bfloat16)
+    g = _gen(20)
+    y[-3:] = torch.randn(3, 2 * ffn, generator=g, device="cuda").bfloat16()
+    assert y.numel() > 2 ** 31
+    s = torch.rand(rows, generator=g, device="cuda")
+    h = ops.swiglu(y, s)
+    assert torch.equal(h[-3:], ops.swiglu(y[-3:].clone(), s[-3:].clone()))
+    dy, ds = ops.swiglu_grad(h, y, s)
+    want = ops.swiglu_grad(h[-3:].clone(), y[-3:].clone(), s[-3:].clone())
+    assert torch.equal(dy[-3:], want[0]) and torch.equal(ds[-3:], want[1])
 
 
 def test_swiglu_strides_and_expanded_gradients():
