@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 8) {
         if (lane == 0) {
+            const uint64_t policy = sm100::l2_evict_first();
             uint32_t issued = 0, stage = 0, phase = 0;
             bool ok = true;
             for (int tile = first_tile; ok && tile < total_tiles && !aborted(); tile += tile_step) {
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     uint8_t* sw = smem + stage * S::kStageBytes;
                     sm100::mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
-                    sm100::tma_load_2d(sw, &tmap_b, &full[stage], kb * kBK, brow0);
+                    sm100::tma_load_2d_hint(sw, &tmap_b, &full[stage], kb * kBK, brow0, policy);
                     sm100::tma_load_2d(sw + S::kWBytes, &tmap_a, &full[stage], kb * kBK, row0);
                     next(stage, phase);
                 }

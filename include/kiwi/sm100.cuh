@@ -82,6 +82,23 @@ KIWI_DEV void tma_load_2d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
         : "memory");
 }
 
+/// An L2 policy for data that is read once.
+KIWI_DEV uint64_t l2_evict_first() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+
+/// tma_load_2d with an L2 policy.
+KIWI_DEV void tma_load_2d_hint(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t x, int32_t y,
+                               uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(
+            smem_addr(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "l"(policy)
+        : "memory");
+}
+
 // ---- cp.async (LDGSTS): per-thread asynchronous global -> shared copies ----
 
 KIWI_DEV void cp_async_16(void* smem_dst, const void* gmem_src) {
