@@ -21,7 +21,8 @@
 // Bound by weight streaming, and for the smallest calls by launch and set-up.
 // Measured on one B200 (graph, warm): 1 row, 7168 x 2048 in 6.9 us; 33 rows,
 // 4096 x 7168 in 13 us; 32 rows for each of 32 experts, 4096 x 7168 (940 MB of
-// weights) in 150 us = 6.3 TB/s.
+// weights) in 142 to 147 us = 6.4 to 6.6 TB/s (2 % more without the evict-first
+// policy on the weights, 5 % with 128-byte instead of 256-byte L2 promotion).
 //
 //   warps 0..7   drain: TMEM lane quadrant = warp % 4, weight block = warp / 4;
 //                then a token's 256 columns a warp
