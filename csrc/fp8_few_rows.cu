@@ -224,13 +224,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float* sa1 = p.a.a_scale + (row + 32 < last ? row + 32 : last) * p.a.a_scale_stride;
             const float* sb0 = p.a.b_scale + (static_cast<int64_t>(g) * p.nb + 2 * nt) * p.k_blocks;
             const float* sb1 = 2 * nt + 1 < p.nb ? sb0 + p.k_blocks : sb0;
-            float a0 = __ldg(sa0 + kb0), a1 = ROWS > 32 ? __ldg(sa1 + kb0) : 0.f;
+            float a0 = ld_a_scale(sa0 + kb0), a1 = ROWS > 32 ? ld_a_scale(sa1 + kb0) : 0.f;
             float b0 = __ldg(sb0 + kb0), b1 = __ldg(sb1 + kb0);
             for (int kb = kb0; kb < kb1; ++kb) {
                 const float v00 = a0 * b0, v01 = a0 * b1, v10 = a1 * b0, v11 = a1 * b1;
                 if (kb + 1 < kb1) {
-                    a0 = __ldg(sa0 + kb + 1);
-                    if (ROWS > 32) a1 = __ldg(sa1 + kb + 1);
+                    a0 = ld_a_scale(sa0 + kb + 1);
+                    if (ROWS > 32) a1 = ld_a_scale(sa1 + kb + 1);
                     b0 = __ldg(sb0 + kb + 1);
                     b1 = __ldg(sb1 + kb + 1);
                 }

@@ -260,12 +260,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float* sa1 = p.a.a_scale + (row + 32 < last ? row + 32 : last) * p.a.a_scale_stride;
                 const float* sb0 = p.a.b_scale + (static_cast<int64_t>(g) * p.nb + 2 * nt) * k_blocks;
                 const float* sb1 = 2 * nt + 1 < p.nb ? sb0 + k_blocks : sb0;
-                float a0 = __ldg(sa0), a1 = __ldg(sa1), b0 = __ldg(sb0), b1 = __ldg(sb1);
+                float a0 = ld_a_scale(sa0), a1 = ld_a_scale(sa1), b0 = __ldg(sb0), b1 = __ldg(sb1);
                 for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                     const float2 v0 = make_float2(a0 * b0, a0 * b1), v1 = make_float2(a1 * b0, a1 * b1);
                     if (kb + 1 < k_blocks) {
-                        a0 = __ldg(sa0 + kb + 1);
-                        a1 = __ldg(sa1 + kb + 1);
+                        a0 = ld_a_scale(sa0 + kb + 1);
+                        a1 = ld_a_scale(sa1 + kb + 1);
                         b0 = __ldg(sb0 + kb + 1);
                         b1 = __ldg(sb1 + kb + 1);
                     }

@@ -75,6 +75,16 @@ __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
 }
 
+/// A scale of A.  Not through the read-only path: in a product that follows
+/// another one, the first may still be writing these while this kernel runs, up
+/// to grid_wait_before(), and what that path reads has to stay as it is for the
+/// whole kernel.
+__device__ __forceinline__ float ld_a_scale(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+
 /// x / (1 + exp(-x)) with the approximate division (2 steps of 2^-23; 0 where
 /// exp(-x) exceeds 2^126): 64 of them are straight-line code in an epilogue, and
 /// with IEEE divisions the SM spent 11 us a tile fetching it.
