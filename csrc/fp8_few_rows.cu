@@ -364,8 +364,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float amax = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
 #pragma unroll
                         for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-                        const float s = amax > 0.f ? amax / ep::kFp8Max : 1.0f;
-                        const float inv = amax > 0.f ? ep::kFp8Max / amax : 0.f;
+                        float s, inv;
+                        ep::fp8_block_scale(amax, s, inv);
                         const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(h[0] * inv, h[1] * inv),
                                                                      __NV_SATFINITE, __NV_E4M3);
                         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(h[2] * inv, h[3] * inv),

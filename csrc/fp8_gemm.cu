@@ -389,8 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         break;
                     }
                     amax = fmaxf(amax, slot[(half ^ 1) * kBM + place]);
-                    const float scale = amax > 0.f ? amax / ep::kFp8Max : 1.0f;
-                    const float inv = amax > 0.f ? ep::kFp8Max / amax : 0.f;
+                    float scale, inv;
+                    ep::fp8_block_scale(amax, scale, inv);
                     uint4 w[4];
                     uint32_t* wi = reinterpret_cast<uint32_t*>(w);
 #pragma unroll
@@ -465,8 +465,8 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_blocks_kernel(const _
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kQuantThreads / 32; ++i) amax = fmaxf(amax, s_max[i]);
-    const float scale = amax > 0.f ? amax / ep::kFp8Max : 1.0f;
-    const float inv = amax > 0.f ? ep::kFp8Max / amax : 0.f;
+    float scale, inv;
+    ep::fp8_block_scale(amax, scale, inv);
     if (threadIdx.x == 0) scales[blockIdx.x] = scale;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -16,6 +16,10 @@ namespace kiwi::ep {
 
 inline constexpr float kFp8Max = 448.0f;
 inline constexpr float kFp4Max = 6.0f;
+/// The smallest amax whose 448 / amax is finite in fp32.  A smaller block is
+/// quantised as if this were its amax (scale 2^-128): with an infinite factor
+/// its zeros would become NaN and its other values +-448.
+inline constexpr float kFp8MinAmax = 0x1.c00002p-120f;
 
 #if defined(__CUDACC__)
 
@@ -40,6 +44,13 @@ KIWI_DEV uint4 f32x8_to_bf16(const float (&f)[8]) {
     return u;
 }
 
+/// Scale and factor of an FP8 block: codes are its values * inv, which stand for code * scale.
+KIWI_DEV void fp8_block_scale(float amax, float& scale, float& inv) {
+    const float a = fmaxf(amax, kFp8MinAmax);
+    scale = amax > 0.f ? a / kFp8Max : 1.0f;
+    inv = amax > 0.f ? kFp8Max / a : 0.f;
+}
+
 /// FP8 1x128: lane covers 16 elements of a 512-element chunk; 8 lanes share a block scale.
 KIWI_DEV void quant_fp8_16(const uint4 (&in)[2], float& scale, uint4& out) {
     float f[16];
@@ -56,8 +67,8 @@ KIWI_DEV void quant_fp8_16(const uint4 (&in)[2], float& scale, uint4& out) {
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 4));
-    scale = amax > 0.f ? amax / kFp8Max : 1.0f;
-    const float inv = amax > 0.f ? kFp8Max / amax : 0.f;
+    float inv;
+    fp8_block_scale(amax, scale, inv);
     uint16_t q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

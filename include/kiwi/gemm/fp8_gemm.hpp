@@ -28,7 +28,7 @@ struct Fp8GemmArgs {
     __nv_bfloat16* c;         // [rows, n] ([rows, n / 2] with swiglu), or null with codes
     int64_t ldc;              // elements
     uint8_t* codes;           // swiglu only: [rows, n / 2] contiguous e4m3 codes, 16-byte aligned, instead of c ...
-    float* scales;            // ... with [rows, n / 256] scales amax / 448 (1 for an all-zero block)
+    float* scales;            // ... with [rows, n / 256] scales amax / 448 (1 for an all-zero block, 2^-128 at the least)
     const float* row_scale;   // optional [rows]: factor of an output row (bf16 output)
     bool swiglu;              // B holds blocks of 128 gate and 128 up rows; n a multiple of 256
     // Two products in a row on a stream, the second on the first's output: the
@@ -45,7 +45,7 @@ void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream);
 
 /// 128 x 128 block quantisation of bf16 w [rows, cols] (row stride ld elements)
 /// to e4m3 codes [rows, cols] (16-byte aligned) and scales [ceil(rows / 128), ceil(cols / 128)] =
-/// amax / 448 (1 for an all-zero block).
+/// amax / 448 (1 for an all-zero block, 2^-128 where 448 / amax would overflow).
 void quant_fp8_blocks(const __nv_bfloat16* w, int64_t ld, int64_t rows, int64_t cols, uint8_t* codes, float* scales,
                       cudaStream_t stream);
 

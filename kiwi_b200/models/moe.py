@@ -18,6 +18,7 @@ import torch
 import torch.nn.functional as F
 
 FP8_MAX = 448.0
+FP8_MIN_AMAX = float.fromhex("0x1.c00002p-120")  # the smallest amax whose 448 / amax is finite in fp32
 FP4_MAX = 6.0
 FP4_VALUES = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
 
@@ -112,15 +113,17 @@ def route_reference(logits, topk):
 def quant_fp8_codes(x, block=128):
     """1 x `block` FP8 e4m3 quantisation of rows of x, the dispatch wire format:
     (codes float8_e4m3fn [t, h], fp32 scales [t, h / block]) with scale =
-    amax / 448 per block (1 for an all-zero block)."""
+    amax / 448 per block (1 for an all-zero block, 2^-128 where amax is below
+    FP8_MIN_AMAX)."""
     t, h = x.shape
     xf = x.float().view(t, h // block, block)
     amax = xf.abs().amax(-1, keepdim=True)
     # Tensor operands keep both divisions IEEE, as on the device (a Python
     # scalar operand makes CUDA multiply by a reciprocal instead).
     fmax = torch.full_like(amax, FP8_MAX)
-    scale = torch.where(amax > 0, amax / fmax, torch.ones_like(amax))
-    inv = torch.where(amax > 0, fmax / amax, torch.zeros_like(amax))  # then multiply by it, as on the device
+    top = amax.clamp(min=FP8_MIN_AMAX)
+    scale = torch.where(amax > 0, top / fmax, torch.ones_like(amax))
+    inv = torch.where(amax > 0, fmax / top, torch.zeros_like(amax))  # then multiply by it, as on the device
     q = (xf * inv).clamp(-FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
     return q.view(t, h), scale.view(t, h // block)
 

@@ -181,7 +181,8 @@ def expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale=N
 
 def quant_fp8_weights(w):
     """(codes float8_e4m3fn [R, K], fp32 scales [ceil(R / 128), ceil(K / 128)]) of a
-    bf16 matrix in 128 x 128 blocks, scale = amax / 448 (1 for an all-zero block).
+    bf16 matrix in 128 x 128 blocks, scale = amax / 448 (1 for an all-zero block;
+    2^-128 where 448 / amax would overflow, amax < 1.4e-36).
     Grouped weights [G * N, K] with N a multiple of 128 quantise group by group."""
     if not w.is_cuda:
         if w.dtype != torch.bfloat16 or w.dim() != 2:

@@ -2,7 +2,8 @@
 kernel's arithmetic:
 
 * ``quant_fp8(x) -> (codes float8_e4m3fn [T, H], fp32 scales [T, H / 128])``,
-  1x128 blocks, scale = amax / 448 per block (1 for an all-zero block);
+  1x128 blocks, scale = amax / 448 per block (1 for an all-zero block; 2^-128
+  where 448 / amax would overflow, amax < 1.4e-36);
 * ``quant_nvfp4(x) -> (packed e2m1 codes uint8 [T, H / 2], scale bytes uint8
   [T, S])``, the NVLink dispatch's NVFP4 wire bytes: an fp32 row scale
   amax / (448 * 6), then one e4m3 scale per 16 elements relative to it, zero

@@ -1,0 +1,83 @@
+"""Edges of the experts' operators on CPU tensors: blocks too small for a finite
+factor, counts past 32 bits, refusals."""
+import pytest
+import torch
+
+from kiwi_b200 import ops
+from kiwi_b200.models import moe
+
+BF16, F32 = 2.0 ** -8, 2.0 ** -23
+FLOOR = float.fromhex("0x1.c00002p-120")  # the smallest amax whose 448 / amax is finite in fp32
+
+
+def _e4m3_close(codes, scale, x):
+    """Quantised values against x (64 bits): half a step is 2^-4 of a value, and
+    2^-10 of the scale below e4m3's normal range.  2^-20 of a value is for the
+    factor's and the scale's own rounding: 2^-24 each, and 2^-22 where the scale
+    is subnormal (2^-128 with steps of 2^-149)."""
+    got = codes.double() * scale
+    assert bool(((got - x).abs() <= (2.0 ** -4 + 2.0 ** -20) * x.abs() + 2.0 ** -10 * scale).all())
+
+
+TINY = [2.0 ** -149, 1e-40, 1e-37, 1.3e-36, FLOOR * (1 - 2.0 ** -24), FLOOR, 2e-36, 1e-35, 1e-30]
+
+
+@pytest.mark.parametrize("amax", TINY, ids=lambda a: f"{a:.3g}")
+def test_rows_of_a_tiny_block(amax):
+    x = torch.zeros(3, 256)
+    x[0, 0], x[0, 5], x[0, 200] = amax, -amax / 3, 1.0
+    x[1, 100] = -amax
+    codes, scales = moe.quant_fp8_codes(x)
+    assert bool((scales > 0).all()) and scales[2, 0] == 1 and bool((codes[x == 0].float() == 0).all())
+    _e4m3_close(codes, scales.double().repeat_interleave(128, 1), x.double())
+    x = x.bfloat16()
+    codes, scales = ops.quant_fp8(x)
+    _e4m3_close(codes, scales.double().repeat_interleave(128, 1), x.double())
+
+
+@pytest.mark.parametrize("amax", TINY, ids=lambda a: f"{a:.3g}")
+def test_weights_of_a_tiny_block(amax):
+    w = torch.zeros(200, 256).bfloat16()
+    w[3, 7], w[100, 100], w[0, 200] = amax, -amax / 3, 1.0
+    codes, scales = ops.quant_fp8_weights(w)
+    assert bool((codes[w == 0].float() == 0).all())
+    s = scales.double().repeat_interleave(128, 0)[:200].repeat_interleave(128, 1)
+    _e4m3_close(codes, s, w.double())
+
+
+def test_blocks_with_a_finite_factor_keep_their_codes():
+    x = torch.randn(64, 256) * torch.exp2(torch.randint(-118, 60, (64, 1)).float())
+    amax = x.view(64, 2, 128).abs().amax(2, keepdim=True)
+    assert float(amax.min()) >= FLOOR
+    codes, scales = moe.quant_fp8_codes(x)
+    want = (x.view(64, 2, 128) * (torch.full_like(amax, 448.0) / amax)).clamp(-448, 448).to(torch.float8_e4m3fn)
+    assert torch.equal(scales, (amax / 448)[:, :, 0]) and torch.equal(codes.float(), want.view(64, 256).float())
+
+
+@pytest.mark.parametrize("magnitude", [1e-18, 1e-19, 3e-20, 1e-20, 1e-21, 1e-22, 1e-23, 1e-37])
+def test_ffn_of_tiny_rows(magnitude):
+    """Against 64 bits of the same codes: gate and up are fp32 sums of K products
+    (K steps of 2^-23 of their magnitudes), each hidden value loses at most 4
+    steps of 2^-149 besides and is quantised once (as above, with a scale of at
+    least 2^-128), the second product's scales round to a step of 2^-149, and the
+    result to bf16 steps of 2^-133 at the least."""
+    torch.manual_seed(1)
+    h, f, rows = 256, 128, 6
+    x = (torch.randn(rows, h) * magnitude).bfloat16()
+    a, sa = ops.quant_fp8(x)
+    w13, s13 = ops.quant_fp8_weights((torch.randn(2 * f, h) * 0.02).bfloat16())
+    w2, s2 = ops.quant_fp8_weights((torch.randn(h, f) * 0.02).bfloat16())
+    out = ops.expert_ffn_fp8(a, sa, w13, s13, w2, s2, [rows])
+    xd = a.double() * sa.double().repeat_interleave(128, 1)
+    wd = w13.double() * s13.double().repeat_interleave(128, 0).repeat_interleave(128, 1)
+    y, e = xd @ wd.T, h * F32 * (xd.abs() @ wd.abs().T)
+    gate, up = y[:, :f], y[:, f:]
+    silu = gate * torch.sigmoid(gate)
+    hid = silu * up
+    d = 1.1 * e[:, :f] * (up.abs() + e[:, f:]) + silu.abs() * e[:, f:] + 16 * F32 * hid.abs() + 4 * 2.0 ** -149
+    w = w2.double() * s2.double().repeat_interleave(128, 0).repeat_interleave(128, 1)
+    ref = hid @ w.T
+    s = ((hid.abs() + d).amax(1, keepdim=True) / 448).clamp(min=2.0 ** -128)
+    each = (2.0 ** -4 + 2.0 ** -20) * (hid.abs() + d) + 2.0 ** -10 * s + d
+    slack = each @ w.abs().T + f * F32 * (hid.abs() + each) @ w.abs().T + f * 448 * 448 * 2.0 ** -149 + 2.0 ** -134
+    assert bool(((out.double() - ref).abs() <= BF16 * ref.abs() + slack).all())

@@ -1,0 +1,80 @@
+"""Edges of the experts' operators on the GPU: blocks too small for a finite
+factor, refusals before a launch, error words, strides and counts that other
+tests do not have."""
+import pytest
+import torch
+
+from kiwi_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = 2.0 ** -8, 2.0 ** -23
+FLOOR = float.fromhex("0x1.c00002p-120")  # the smallest amax whose 448 / amax is finite in fp32
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _fp8(g, rows, k, mag=1.0):
+    """Quantised bf16 rows and their 64-bit values."""
+    x = (torch.randn(rows, k, generator=g, device="cuda") * mag).bfloat16()
+    codes, s = ops.quant_fp8(x)
+    return codes, s, codes.double() * s.double().repeat_interleave(128, 1)
+
+
+def _fp8_weights(g, rows, k, mag=0.02):
+    codes, s = ops.quant_fp8_weights((torch.randn(rows, k, generator=g, device="cuda") * mag).bfloat16())
+    return codes, s, codes.double() * s.double().repeat_interleave(128, 0)[:rows].repeat_interleave(128, 1)[:, :k]
+
+
+def _e4m3_close(codes, scale, x, slack=0.0):
+    """Quantised values against x (64 bits): half a step is 2^-4 of a value, and
+    2^-10 of the scale below e4m3's normal range.  2^-20 of a value is for the
+    factor's and the scale's own rounding: 2^-24 each, and 2^-22 where the scale
+    is subnormal (2^-128 with steps of 2^-149)."""
+    got = codes.double() * scale
+    assert bool(((got - x).abs() <= (2.0 ** -4 + 2.0 ** -20) * x.abs() + 2.0 ** -10 * scale + slack).all())
+
+
+@pytest.mark.parametrize("amax", [2.0 ** -133, 1e-37, 1.3e-36, FLOOR, 1e-35, 1e-30], ids=lambda a: f"{a:.3g}")
+def test_tiny_blocks(amax):
+    x = torch.zeros(200, 512, device="cuda")
+    x[0, 0], x[0, 5], x[0, 200], x[1, 300], x[150, 400] = amax, -amax / 3, 1.0, -amax, amax
+    x = x.bfloat16()
+    codes, scales = ops.quant_fp8(x)
+    assert bool((codes[x == 0].float() == 0).all()) and scales[2, 0] == 1
+    _e4m3_close(codes, scales.double().repeat_interleave(128, 1), x.double())
+    codes, scales = ops.quant_fp8_weights(x)
+    assert bool((codes[x == 0].float() == 0).all())
+    _e4m3_close(codes, scales.double().repeat_interleave(128, 0)[:200].repeat_interleave(128, 1), x.double())
+
+
+@pytest.mark.parametrize("magnitude", [1e-18, 1e-19, 1e-20, 1e-21, 1e-22, 1e-37])
+@pytest.mark.parametrize("rows", [3, 2000])  # both kernels
+def test_hidden_rows_of_a_tiny_block(rows, magnitude):
+    g = _gen(rows)
+    k, f = 256, 256
+    a, sa, x = _fp8(g, rows, k, magnitude)
+    b, sb, w = _fp8_weights(g, 2 * f, k)
+    b[:1] = 0  # a zero gate row: a zero hidden column in each block
+    w[:1] = 0
+    cnt = torch.tensor([rows], dtype=torch.int32, device="cuda")
+    codes, scales = ops.grouped_fp8_swiglu(a, sa, b, sb, cnt)
+    # gate and up: fp32 sums of K products; the approximate exponential and
+    # division cost 16 steps at such gates, underflow 4 steps of 2^-149.
+    y, e = x @ w.T, k * F32 * (x.abs() @ w.abs().T)
+    y, e = (t.view(rows, f // 128, 2, 128) for t in (y, e))
+    gate, up = y[:, :, 0], y[:, :, 1]
+    silu = gate * torch.sigmoid(gate)
+    h = silu * up
+    d = 1.1 * e[:, :, 0] * (up.abs() + e[:, :, 1]) + silu.abs() * e[:, :, 1] + 16 * F32 * h.abs() + 4 * 2.0 ** -149
+    _e4m3_close(codes, scales.double().repeat_interleave(128, 1), h.flatten(1), 1.1 * d.flatten(1))
+    assert bool((codes[:, 0].float() == 0).all())
+    w2, s2, _ = _fp8_weights(g, 256, f)
+    out = ops.expert_ffn_fp8(a, sa, b, sb, w2, s2, cnt)
+    assert bool(torch.isfinite(out).all())
+    assert torch.equal(out, ops.grouped_fp8_gemm(codes, scales, w2, s2, cnt))
+    ops.check_gemm()
