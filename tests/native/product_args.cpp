@@ -1,0 +1,68 @@
+// Argument checks of the C++ entries of the experts' products (no GPU needed):
+// prints "case: message" for each refused call.  No pointer passed here is ever
+// dereferenced, and nothing can be launched: the number of SMs, which every
+// launch asks for first, is refused by this file.
+#include <cstdint>
+#include <cstdio>
+#include <functional>
+
+#include "kiwi/common.hpp"
+#include "kiwi/gemm/fp8_gemm.hpp"
+#include "kiwi/gemm/grouped_gemm.hpp"
+
+namespace kiwi::gemm {
+int num_sms() { throw kiwi::error("accepted"); }
+}  // namespace kiwi::gemm
+
+namespace {
+
+template <typename T>
+T* at(uintptr_t address) {
+    return reinterpret_cast<T*>(address);
+}
+
+constexpr uintptr_t kBase = 1 << 20;  // 16-byte aligned, never dereferenced
+
+kiwi::gemm::Fp8GemmArgs fp8_args() {
+    kiwi::gemm::Fp8GemmArgs a{};
+    a.a = at<uint8_t>(kBase);
+    a.lda = 256;
+    a.b = at<uint8_t>(kBase);
+    a.ldb = 256;
+    a.a_scale = at<float>(kBase);
+    a.a_scale_stride = 2;
+    a.b_scale = at<float>(kBase);
+    a.counts = at<int32_t>(kBase);
+    a.num_groups = 2;
+    a.n = 256;
+    a.k = 256;
+    a.rows = 8;
+    a.c = at<__nv_bfloat16>(kBase);
+    a.ldc = 256;
+    return a;
+}
+
+void report(const char* name, const std::function<void()>& call) {
+    try {
+        call();
+        std::printf("%s: returned\n", name);
+    } catch (const std::exception& e) {
+        std::printf("%s: %s\n", name, e.what());
+    }
+}
+
+void fp8(const char* name, const std::function<void(kiwi::gemm::Fp8GemmArgs&)>& change) {
+    kiwi::gemm::Fp8GemmArgs a = fp8_args();
+    change(a);
+    report(name, [&] { kiwi::gemm::fp8_gemm(a, nullptr); });
+}
+
+}  // namespace
+
+int main() {
+    fp8("fp8 groups without counts", [](auto& a) { a.counts = nullptr; });
+    fp8("fp8 no groups", [](auto& a) { a.num_groups = 0; });
+    fp8("fp8 no output", [](auto& a) { a.c = nullptr; });
+    fp8("fp8 k", [](auto& a) { a.k = 250; });
+    return 0;
+}
