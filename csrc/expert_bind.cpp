@@ -45,7 +45,7 @@ void check_fp8_operand(const torch::Tensor& x, const torch::Tensor& s, int64_t s
     require(x.is_cuda() && x.device() == dev && s.device() == dev, w + " and its scales must be on one CUDA device");
     require(x.scalar_type() == torch::kFloat8_e4m3fn && x.dim() == 2, w + " must be float8_e4m3fn [rows, K]");
     require(x.size(1) >= 16 && x.size(1) % 16 == 0, "K must be a positive multiple of 16");
-    require(x.size(1) < (int64_t{1} << 31), "fewer than 2^31 columns");
+    require(x.size(1) <= INT32_MAX - 256, "K must be below 2^31 - 256");
     require(s.scalar_type() == torch::kFloat32 && s.dim() == 2 && s.size(0) == scale_rows &&
                 s.size(1) == (x.size(1) + 127) / 128,
             w + "'s scales must be fp32 [" + std::to_string(scale_rows) + ", " +
@@ -236,7 +236,7 @@ gemm::GroupedLinearArgs linear_args(int64_t rows, int64_t n, int64_t k, const to
                                     const torch::Device& dev) {
     check_counts(counts, dev);
     require(n >= 64 && n % 64 == 0 && k >= 64 && k % 64 == 0, "N and K must be multiples of 64");
-    require(k < (int64_t{1} << 31) - 256, "fewer than 2^31 columns");
+    require(k <= INT32_MAX - 256, "K must be below 2^31 - 256");
     require(rows < (int64_t{1} << 31) - 256 && counts.numel() * n < (int64_t{1} << 31) - 256, "fewer than 2^31 rows");
     gemm::GroupedLinearArgs a{};
     a.counts = counts.data_ptr<int32_t>();

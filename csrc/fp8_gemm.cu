@@ -578,6 +578,7 @@ void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream) {
     if (args.num_groups < 1 || args.num_groups > kMaxGroups) throw kiwi::error("fp8_gemm: 1..1024 groups");
     if (!args.counts && args.num_groups != 1) throw kiwi::error("fp8_gemm: several groups need counts");
     if (args.n < 1 || args.k < 16 || args.k % 16 != 0) throw kiwi::error("fp8_gemm: K must be a positive multiple of 16");
+    if (args.k > INT32_MAX - 256) throw kiwi::error("fp8_gemm: K must be below 2^31 - 256");
     if (args.num_groups > 1 && args.n % 128 != 0) throw kiwi::error("fp8_gemm: grouped N must be a multiple of 128");
     if (args.swiglu && args.n % kBN != 0) throw kiwi::error("fp8_gemm: SwiGLU needs N to be a multiple of 256");
     if (args.codes && !args.swiglu) throw kiwi::error("fp8_gemm: FP8 output needs swiglu");

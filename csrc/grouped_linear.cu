@@ -423,6 +423,7 @@ CUtensorMap bf16_map(const __nv_bfloat16* ptr, int64_t rows, int64_t cols, int64
 void check(const GroupedLinearArgs& a) {
     if (a.num_groups < 1 || a.num_groups > kMaxGroups) throw kiwi::error("grouped_linear: 1..1024 groups");
     if (a.n < 64 || a.n % 64 || a.k < 64 || a.k % 64) throw kiwi::error("grouped_linear: N and K must be multiples of 64");
+    if (a.k > INT32_MAX - 256) throw kiwi::error("grouped_linear: K must be below 2^31 - 256");
     if (!a.counts || (!a.out && a.rows > 0)) throw kiwi::error("grouped_linear: counts and out are required");
     if (a.rows < 0 || a.rows > INT32_MAX - 256 || static_cast<int64_t>(a.num_groups) * a.n > INT32_MAX - 256) {
         throw kiwi::error("grouped_linear: more than 2^31 rows");

@@ -34,6 +34,7 @@ from .grouped_gemm import _swiglu_tiles
 
 _BLOCK = 128
 _FP8 = torch.float8_e4m3fn
+_MAX_COLUMNS = 2 ** 31 - 257  # the kernels count blocks of columns in 32 bits
 _ops = None
 
 
@@ -52,6 +53,8 @@ def _check_operand(x, s, scale_rows, what):
         raise ValueError(f"{what} must be float8_e4m3fn [rows, K]")
     if x.shape[1] < 16 or x.shape[1] % 16:
         raise ValueError("K must be a positive multiple of 16")
+    if x.shape[1] > _MAX_COLUMNS:
+        raise ValueError("K must be below 2^31 - 256")
     want = (scale_rows, -(-x.shape[1] // _BLOCK))
     if s.dtype != torch.float32 or tuple(s.shape) != want:
         raise ValueError(f"{what}'s scales must be fp32 {list(want)}")

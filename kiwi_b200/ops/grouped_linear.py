@@ -32,7 +32,7 @@ Gradients are once differentiable.
 """
 import torch
 
-from .fp8_gemm import _as_counts, _checked_sum, _native_ops
+from .fp8_gemm import _MAX_COLUMNS, _as_counts, _checked_sum, _native_ops
 from .grouped_gemm import grouped_gemm_reference
 
 
@@ -42,6 +42,8 @@ def _check(x, w_rows, w_cols, groups, what):
     n = w_rows // groups
     if n < 64 or n % 64 or w_cols < 64 or w_cols % 64:
         raise ValueError("N and K must be multiples of 64")
+    if w_cols > _MAX_COLUMNS:
+        raise ValueError("K must be below 2^31 - 256")
 
 
 def _check_counts(counts):

@@ -9,6 +9,7 @@
 #include "kiwi/common.hpp"
 #include "kiwi/gemm/fp8_gemm.hpp"
 #include "kiwi/gemm/grouped_gemm.hpp"
+#include "kiwi/gemm/grouped_linear.hpp"
 
 namespace kiwi::gemm {
 int num_sms() { throw kiwi::error("accepted"); }
@@ -57,6 +58,21 @@ void fp8(const char* name, const std::function<void(kiwi::gemm::Fp8GemmArgs&)>& 
     report(name, [&] { kiwi::gemm::fp8_gemm(a, nullptr); });
 }
 
+void linear(const char* name, void (*entry)(const kiwi::gemm::GroupedLinearArgs&, cudaStream_t),
+            const std::function<void(kiwi::gemm::GroupedLinearArgs&)>& change) {
+    kiwi::gemm::GroupedLinearArgs a{};
+    a.x = a.w = a.dy = at<__nv_bfloat16>(kBase);
+    a.ldx = a.ldw = a.lddy = a.ldo = 256;
+    a.out = at<void>(kBase);
+    a.counts = at<int32_t>(kBase);
+    a.num_groups = 2;
+    a.n = 256;
+    a.k = 256;
+    a.rows = 8;
+    change(a);
+    report(name, [&] { entry(a, nullptr); });
+}
+
 }  // namespace
 
 int main() {
@@ -64,5 +80,9 @@ int main() {
     fp8("fp8 no groups", [](auto& a) { a.num_groups = 0; });
     fp8("fp8 no output", [](auto& a) { a.c = nullptr; });
     fp8("fp8 k", [](auto& a) { a.k = 250; });
+    fp8("fp8 large k", [](auto& a) { a.k = INT32_MAX - 15; });
+    linear("forward large k", kiwi::gemm::grouped_linear_forward, [](auto& a) { a.k = INT32_MAX - 63; });
+    linear("dgrad large k", kiwi::gemm::grouped_linear_dgrad, [](auto& a) { a.k = INT32_MAX - 63; });
+    linear("wgrad large k", kiwi::gemm::grouped_linear_wgrad, [](auto& a) { a.k = INT32_MAX - 63; });
     return 0;
 }

@@ -81,3 +81,15 @@ def test_ffn_of_tiny_rows(magnitude):
     each = (2.0 ** -4 + 2.0 ** -20) * (hid.abs() + d) + 2.0 ** -10 * s + d
     slack = each @ w.abs().T + f * F32 * (hid.abs() + each) @ w.abs().T + f * 448 * 448 * 2.0 ** -149 + 2.0 ** -134
     assert bool(((out.double() - ref).abs() <= BF16 * ref.abs() + slack).all())
+
+
+def test_rows_too_long_for_32_bits():
+    """Meta tensors: the check comes before any arithmetic."""
+    k = 2 ** 31 - 16
+    a = torch.empty(1, k, dtype=torch.float8_e4m3fn, device="meta")
+    s = torch.empty(1, -(-k // 128), device="meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.fp8_gemm(a, s, a, s)
+    x = torch.empty(64, 2 ** 31 - 64, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.grouped_linear(x, x, torch.tensor([64]))

@@ -78,3 +78,15 @@ def test_hidden_rows_of_a_tiny_block(rows, magnitude):
     assert bool(torch.isfinite(out).all())
     assert torch.equal(out, ops.grouped_fp8_gemm(codes, scales, w2, s2, cnt))
     ops.check_gemm()
+
+
+def test_rows_too_long_for_32_bits():
+    """Refused before anything is allocated or launched (the operands are one element each)."""
+    k = 2 ** 31 - 16
+    a = torch.zeros(1, 1, device="cuda").to(torch.float8_e4m3fn).expand(1, k)
+    s = torch.ones(1, 1, device="cuda").expand(1, -(-k // 128))
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.fp8_gemm(a, s, a, s)
+    x = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(64, 2 ** 31 - 64)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.grouped_linear(x, x, torch.tensor([64], dtype=torch.int32, device="cuda"))

@@ -9,7 +9,7 @@ import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 NVCC = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-SOURCES = ["csrc/fp8_gemm.cu", "csrc/fp8_few_rows.cu", "csrc/tensor_map.cpp", "src/p2p/driver.cpp",
+SOURCES = ["csrc/fp8_gemm.cu", "csrc/fp8_few_rows.cu", "csrc/grouped_linear.cu", "csrc/tensor_map.cpp", "src/p2p/driver.cpp",
            "tests/native/product_args.cpp"]
 
 
@@ -40,6 +40,10 @@ def refusals(tmp_path_factory):
     ("fp8 no groups", "1..1024 groups"),
     ("fp8 no output", "missing operands or output"),
     ("fp8 k", "multiple of 16"),
+    ("fp8 large k", "2^31"),
+    ("forward large k", "2^31"),
+    ("dgrad large k", "2^31"),
+    ("wgrad large k", "2^31"),
 ])
 def test_refused_before_a_device_is_touched(refusals, case, words):
     assert words in refusals[case], refusals[case]
