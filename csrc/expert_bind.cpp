@@ -200,12 +200,14 @@ torch::Tensor expert_ffn_fp8_py(torch::Tensor x, torch::Tensor x_scale, torch::T
             "w13 must be [E * 2F, H] and w2 [E * H, F]");
     const c10::cuda::CUDAGuard guard(x.device());
     // The second product's arguments are refused before the first is launched.
+    check_row_scale(row_scale, x.size(0), x.device());
     if (out) {
         check_out(*out, x.size(0), x.size(1), torch::kBFloat16, x.device());
         for (const auto& t : {x, x_scale, w13, w13_scale, w2, w2_scale})
             require(!overlap(*out, t), "out must not overlap an input");
+        if (row_scale) require(!overlap(*out, *row_scale), "out must not overlap an input");
     }
-    check_row_scale(row_scale, x.size(0), x.device());
+    require(w2.size(0) < (int64_t{1} << 31) - 256, "fewer than 2^31 rows");
     require(x.size(1) % 128 == 0, "H must be a multiple of 128");
     check_fp8_operand(w2, w2_scale, w2.size(0) / 128, x.device(), "w2");
     auto h = fp8_swiglu_quant(x, x_scale, w13, w13_scale, counts, false, true);

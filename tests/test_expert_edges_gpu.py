@@ -90,3 +90,18 @@ def test_rows_too_long_for_32_bits():
     x = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(64, 2 ** 31 - 64)
     with pytest.raises(ValueError, match="2\\^31"):
         ops.grouped_linear(x, x, torch.tensor([64], dtype=torch.int32, device="cuda"))
+
+
+def test_ffn_refuses_an_out_over_its_row_scale_before_it_launches():
+    g = _gen(3)
+    a, sa, _ = _fp8(g, 8, 256)
+    w13, s13, _ = _fp8_weights(g, 256, 256)
+    w2, s2, _ = _fp8_weights(g, 256, 128)
+    buf = torch.zeros(8 * 256 + 16, device="cuda", dtype=torch.bfloat16)
+    out, scale = buf[:8 * 256].view(8, 256), buf[-24:-8].view(torch.float32)
+    # Counts that a launched product reports: nothing may have run.
+    cnt = torch.tensor([9], dtype=torch.int32, device="cuda")
+    ops.check_gemm()
+    with pytest.raises(ValueError, match="overlap"):
+        ops.expert_ffn_fp8(a, sa, w13, s13, w2, s2, cnt, row_scale=scale, out=out)
+    ops.check_gemm()
