@@ -144,6 +144,7 @@ torch::Tensor fp8_gemm_out(torch::Tensor a, torch::Tensor a_scale, torch::Tensor
         check_out(*out, a.size(0), cols, torch::kBFloat16, a.device());
         for (const auto& t : {a, a_scale, b, b_scale}) require(!overlap(*out, t), "out must not overlap an input");
         if (row_scale) require(!overlap(*out, *row_scale), "out must not overlap an input");
+        if (counts) require(!overlap(*out, *counts), "out must not overlap an input");
         o = *out;
     } else {
         o = torch::empty({a.size(0), cols}, a.options().dtype(torch::kBFloat16));
@@ -203,7 +204,7 @@ torch::Tensor expert_ffn_fp8_py(torch::Tensor x, torch::Tensor x_scale, torch::T
     check_row_scale(row_scale, x.size(0), x.device());
     if (out) {
         check_out(*out, x.size(0), x.size(1), torch::kBFloat16, x.device());
-        for (const auto& t : {x, x_scale, w13, w13_scale, w2, w2_scale})
+        for (const auto& t : {x, x_scale, w13, w13_scale, w2, w2_scale, counts})
             require(!overlap(*out, t), "out must not overlap an input");
         if (row_scale) require(!overlap(*out, *row_scale), "out must not overlap an input");
     }
@@ -268,7 +269,7 @@ torch::Tensor linear_forward_py(torch::Tensor x, torch::Tensor w, torch::Tensor 
             "w must be [groups * N, K] with x's K");
     auto a = linear_args(x.size(0), w.size(0) / counts.numel(), x.size(1), counts, x.device());
     const torch::Tensor xr = tma_rows(x), wr = tma_rows(w);
-    torch::Tensor o = linear_out(out, x.size(0), a.n, torch::kBFloat16, x, {x, w});
+    torch::Tensor o = linear_out(out, x.size(0), a.n, torch::kBFloat16, x, {x, w, counts});
     a.x = bf16_ptr(xr);
     a.ldx = row_stride(xr);
     a.w = bf16_ptr(wr);
@@ -288,7 +289,7 @@ torch::Tensor linear_dgrad_py(torch::Tensor dy, torch::Tensor w, torch::Tensor c
     require(counts.numel() >= 1 && w.size(0) == counts.numel() * dy.size(1), "w must be [groups * N, K] with dy's N");
     auto a = linear_args(dy.size(0), dy.size(1), w.size(1), counts, dy.device());
     const torch::Tensor dr = tma_rows(dy), wr = tma_rows(w);
-    torch::Tensor o = linear_out(out, dy.size(0), a.k, torch::kBFloat16, dy, {dy, w});
+    torch::Tensor o = linear_out(out, dy.size(0), a.k, torch::kBFloat16, dy, {dy, w, counts});
     a.dy = bf16_ptr(dr);
     a.lddy = row_stride(dr);
     a.w = bf16_ptr(wr);
@@ -312,7 +313,7 @@ torch::Tensor linear_wgrad_py(torch::Tensor dy, torch::Tensor x, torch::Tensor c
     require(type == torch::kBFloat16 || type == torch::kFloat32, "out must be bf16 or fp32");
     auto a = linear_args(dy.size(0), dy.size(1), x.size(1), counts, dy.device());
     const torch::Tensor dr = tma_rows(dy), xr = tma_rows(x);
-    torch::Tensor o = linear_out(out, counts.numel() * a.n, a.k, type, dy, {dy, x});
+    torch::Tensor o = linear_out(out, counts.numel() * a.n, a.k, type, dy, {dy, x, counts});
     a.dy = bf16_ptr(dr);
     a.lddy = row_stride(dr);
     a.x = bf16_ptr(xr);

@@ -105,3 +105,24 @@ def test_ffn_refuses_an_out_over_its_row_scale_before_it_launches():
     with pytest.raises(ValueError, match="overlap"):
         ops.expert_ffn_fp8(a, sa, w13, s13, w2, s2, cnt, row_scale=scale, out=out)
     ops.check_gemm()
+
+
+def test_out_over_the_counts_is_refused():
+    """Every CTA reads the counts for itself: an out written over them would
+    change the schedule under the CTAs that start later."""
+    g = _gen(6)
+    a, sa, _ = _fp8(g, 8, 256)
+    w13, s13, _ = _fp8_weights(g, 256, 256)
+    w2, s2, _ = _fp8_weights(g, 256, 128)
+    x, w = torch.zeros(8, 256, device="cuda").bfloat16(), torch.zeros(256, 256, device="cuda").bfloat16()
+    buf = torch.zeros(256 * 256, device="cuda", dtype=torch.bfloat16)
+    out, cnt = buf[:8 * 256].view(8, 256), buf[:2].view(torch.int32)
+    for f in (lambda: ops.grouped_fp8_gemm(a, sa, w13, s13, cnt, out=out),
+              lambda: ops.grouped_fp8_gemm(a, sa, w13, s13, cnt, out=out[:, :128], swiglu=True),
+              lambda: ops.expert_ffn_fp8(a, sa, w13, s13, w2, s2, cnt, out=out),
+              lambda: ops.grouped_linear(x, w, cnt, out=out),
+              lambda: ops.grouped_linear_dgrad(x, w, cnt, out=out),
+              lambda: ops.grouped_linear_wgrad(x, x, cnt, out=buf.view(256, 256))):
+        with pytest.raises(ValueError, match="overlap"):
+            f()
+    assert int(cnt) == 0
