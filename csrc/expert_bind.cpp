@@ -424,19 +424,13 @@ struct SwiGLU : torch::autograd::Function<SwiGLU> {
     }
 };
 
-/// Reads and clears a device's error word (waits for the current stream).
+/// Takes and clears a device's error word (waits for the current stream).
 int64_t gemm_error(int64_t device) {
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
-    uint32_t* word = gemm::gemm_error_word();
-    uint32_t v = 0;
-    cudaStream_t s = cur_stream();
-    C10_CUDA_CHECK(cudaMemcpyAsync(&v, word, sizeof(v), cudaMemcpyDeviceToHost, s));
-    C10_CUDA_CHECK(cudaStreamSynchronize(s));
-    if (v) {
-        C10_CUDA_CHECK(cudaMemsetAsync(word, 0, sizeof(v), s));
-        C10_CUDA_CHECK(cudaStreamSynchronize(s));
-    }
-    return v;
+    const torch::Tensor bits =
+        torch::empty({1}, torch::dtype(torch::kInt32).device(torch::kCUDA, static_cast<c10::DeviceIndex>(device)));
+    gemm::take_error(gemm::gemm_error_word(), reinterpret_cast<uint32_t*>(bits.data_ptr<int32_t>()), cur_stream());
+    return bits.item<int32_t>();
 }
 
 }  // namespace

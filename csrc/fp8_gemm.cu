@@ -494,6 +494,8 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_blocks_kernel(const _
 
 __device__ uint32_t g_error;
 
+__global__ void take_error_kernel(uint32_t* word, uint32_t* out) { *out = atomicExch(word, 0u); }
+
 template <int EPI>
 void launch(const Params& p, cudaStream_t stream) {
     static std::atomic<uint64_t> attr{0};
@@ -572,6 +574,12 @@ uint32_t* gemm_error_word() {
         ptr[dev] = static_cast<uint32_t*>(q);
     }
     return ptr[dev];
+}
+
+void take_error(uint32_t* word, uint32_t* out, cudaStream_t stream) {
+    if (!word || !out) throw kiwi::error("take_error: missing words");
+    take_error_kernel<<<1, 1, 0, stream>>>(word, out);
+    KIWI_CUDA_CHECK(cudaGetLastError());
 }
 
 void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream) {

@@ -53,4 +53,8 @@ void quant_fp8_blocks(const __nv_bfloat16* w, int64_t ld, int64_t rows, int64_t 
 /// group_table.cuh).  Sticky until cleared.
 uint32_t* gemm_error_word();
 
+/// *out = the error word's bits, which are cleared in the same step: a bit that a
+/// kernel on another stream sets meanwhile is either in *out or still in the word.
+void take_error(uint32_t* word, uint32_t* out, cudaStream_t stream);
+
 }  // namespace kiwi::gemm

@@ -126,3 +126,22 @@ def test_out_over_the_counts_is_refused():
         with pytest.raises(ValueError, match="overlap"):
             f()
     assert int(cnt) == 0
+
+
+def test_error_word_is_taken_in_one_step():
+    """Read and cleared by one kernel: with a copy and then a memset, a bit that a
+    product on another stream sets between the two would be lost."""
+    from torch.profiler import ProfilerActivity, profile
+
+    g = _gen(4)
+    a, sa, _ = _fp8(g, 8, 128)
+    b, sb, _ = _fp8_weights(g, 256, 128)
+    ops.check_gemm()
+    ops.grouped_fp8_gemm(a, sa, b, sb, torch.tensor([9], dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        with pytest.raises(RuntimeError, match="counts"):
+            ops.check_gemm()
+    names = [e.name for e in p.events()]
+    assert any("take_error" in n for n in names) and not any("emset" in n for n in names), names
+    ops.check_gemm()
