@@ -93,6 +93,12 @@ bool overlap(const torch::Tensor& x, const torch::Tensor& y) {
     return x0 < y1 && y0 < x1;
 }
 
+uint32_t* error_word(const torch::Tensor& t, const torch::Device& dev) {
+    require(t.device() == dev && t.scalar_type() == torch::kInt32 && t.numel() == 1,
+            "error must be an int32 tensor of one element on the rows' device");
+    return reinterpret_cast<uint32_t*>(t.data_ptr<int32_t>());
+}
+
 struct Fp8Call {
     torch::Tensor a, a_scale, b, b_scale;  // kept alive until the launch
     gemm::Fp8GemmArgs args{};
@@ -132,7 +138,8 @@ Fp8Call fp8_call(const torch::Tensor& a, const torch::Tensor& a_scale, const tor
 }
 
 torch::Tensor fp8_gemm_out(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
-                           OptTensor counts, OptTensor out, bool swiglu, OptTensor row_scale, bool follows) {
+                           OptTensor counts, OptTensor out, bool swiglu, OptTensor row_scale, bool follows,
+                           uint32_t* error) {
     require(a.is_cuda(), "A must be a CUDA tensor");
     const c10::cuda::CUDAGuard guard(a.device());
     Fp8Call c = fp8_call(a, a_scale, b, b_scale, counts);
@@ -155,6 +162,7 @@ torch::Tensor fp8_gemm_out(torch::Tensor a, torch::Tensor a_scale, torch::Tensor
     c.args.swiglu = swiglu;
     c.args.zero_tail = !out && counts;
     c.args.follows = follows;
+    c.args.error = error;
     gemm::fp8_gemm(c.args, cur_stream());
     if (out) written(o);
     return o;
@@ -162,14 +170,14 @@ torch::Tensor fp8_gemm_out(torch::Tensor a, torch::Tensor a_scale, torch::Tensor
 
 torch::Tensor fp8_gemm_py(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
                           OptTensor counts, OptTensor out, bool swiglu, OptTensor row_scale) {
-    return fp8_gemm_out(a, a_scale, b, b_scale, counts, out, swiglu, row_scale, false);
+    return fp8_gemm_out(a, a_scale, b, b_scale, counts, out, swiglu, row_scale, false, nullptr);
 }
 
 /// The gate and up product with its SwiGLU rows quantised to FP8.
 std::pair<torch::Tensor, torch::Tensor> fp8_swiglu_quant(const torch::Tensor& a, const torch::Tensor& a_scale,
                                                          const torch::Tensor& b, const torch::Tensor& b_scale,
                                                          const torch::Tensor& counts, bool zero_tail,
-                                                         bool feeds_next) {
+                                                         bool feeds_next, uint32_t* error) {
     Fp8Call c = fp8_call(a, a_scale, b, b_scale, counts);
     require(c.args.n % 256 == 0, "SwiGLU needs N to be a multiple of 256");
     torch::Tensor codes = torch::empty({a.size(0), c.args.n / 2}, a.options());
@@ -179,6 +187,7 @@ std::pair<torch::Tensor, torch::Tensor> fp8_swiglu_quant(const torch::Tensor& a,
     c.args.swiglu = true;
     c.args.zero_tail = zero_tail;
     c.args.feeds_next = feeds_next;
+    c.args.error = error;
     gemm::fp8_gemm(c.args, cur_stream());
     return {codes, scales};
 }
@@ -187,13 +196,13 @@ py::tuple fp8_swiglu_py(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b,
                         torch::Tensor counts) {
     require(a.is_cuda(), "A must be a CUDA tensor");
     const c10::cuda::CUDAGuard guard(a.device());
-    auto r = fp8_swiglu_quant(a, a_scale, b, b_scale, counts, true, false);
+    auto r = fp8_swiglu_quant(a, a_scale, b, b_scale, counts, true, false, nullptr);
     return py::make_tuple(r.first, r.second);
 }
 
 torch::Tensor expert_ffn_fp8_py(torch::Tensor x, torch::Tensor x_scale, torch::Tensor w13, torch::Tensor w13_scale,
                                 torch::Tensor w2, torch::Tensor w2_scale, torch::Tensor counts, OptTensor row_scale,
-                                OptTensor out) {
+                                OptTensor out, OptTensor error) {
     require(x.is_cuda() && x.dim() == 2, "x must be a CUDA tensor [rows, H]");
     const int64_t groups = counts.numel();
     require(groups >= 1 && w13.dim() == 2 && w2.dim() == 2 && w13.size(0) % (2 * groups) == 0 &&
@@ -211,8 +220,9 @@ torch::Tensor expert_ffn_fp8_py(torch::Tensor x, torch::Tensor x_scale, torch::T
     require(w2.size(0) < (int64_t{1} << 31) - 256, "fewer than 2^31 rows");
     require(x.size(1) % 128 == 0, "H must be a multiple of 128");
     check_fp8_operand(w2, w2_scale, w2.size(0) / 128, x.device(), "w2");
-    auto h = fp8_swiglu_quant(x, x_scale, w13, w13_scale, counts, false, true);
-    return fp8_gemm_out(h.first, h.second, w2, w2_scale, counts, out, false, row_scale, true);
+    uint32_t* word = error ? error_word(*error, x.device()) : nullptr;
+    auto h = fp8_swiglu_quant(x, x_scale, w13, w13_scale, counts, false, true, word);
+    return fp8_gemm_out(h.first, h.second, w2, w2_scale, counts, out, false, row_scale, true, word);
 }
 
 py::tuple quant_fp8_weights_py(torch::Tensor w) {
@@ -424,12 +434,11 @@ struct SwiGLU : torch::autograd::Function<SwiGLU> {
     }
 };
 
-/// Takes and clears a device's error word (waits for the current stream).
-int64_t gemm_error(int64_t device) {
-    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
-    const torch::Tensor bits =
-        torch::empty({1}, torch::dtype(torch::kInt32).device(torch::kCUDA, static_cast<c10::DeviceIndex>(device)));
-    gemm::take_error(gemm::gemm_error_word(), reinterpret_cast<uint32_t*>(bits.data_ptr<int32_t>()), cur_stream());
+/// Reads and clears an error word, or a device's (waits for the current stream).
+int64_t take_error(const torch::Device& dev, uint32_t* word) {
+    const c10::cuda::CUDAGuard guard(dev);
+    const torch::Tensor bits = torch::empty({1}, torch::dtype(torch::kInt32).device(dev));
+    gemm::take_error(word ? word : gemm::gemm_error_word(), reinterpret_cast<uint32_t*>(bits.data_ptr<int32_t>()), cur_stream());
     return bits.item<int32_t>();
 }
 
@@ -445,7 +454,8 @@ void register_expert_ops(py::module_& m) {
           py::arg("counts"), "Grouped FP8 product with SwiGLU, its rows quantised 1x128: (codes, scales).");
     o.def("expert_ffn_fp8", &expert_ffn_fp8_py, py::arg("x"), py::arg("x_scale"), py::arg("w13"), py::arg("w13_scale"),
           py::arg("w2"), py::arg("w2_scale"), py::arg("counts"), py::arg("row_scale") = py::none(),
-          py::arg("out") = py::none(), "The experts' SwiGLU FFN on FP8 rows and weights (two launches).");
+          py::arg("out") = py::none(), py::arg("error") = py::none(),
+          "The experts' SwiGLU FFN on FP8 rows and weights (two launches); errors go into `error` (int32 [1]) if given.");
     o.def("quant_fp8_weights", &quant_fp8_weights_py, py::arg("w"),
           "128x128 FP8 e4m3 quantisation of a bf16 matrix: (codes, fp32 scales).");
     o.def("grouped_linear", [](torch::Tensor x, torch::Tensor w, torch::Tensor counts) {
@@ -463,5 +473,11 @@ void register_expert_ops(py::module_& m) {
           "row_scale * silu(gate) * up of rows in blocks of 128 gate and 128 up columns; differentiable.");
     o.def("swiglu_grad", &swiglu_grad, py::arg("dh"), py::arg("y"), py::arg("row_scale") = py::none(),
           py::arg("need_scale_grad") = false, "(dy, drow_scale or None) of swiglu.");
-    o.def("gemm_error", &gemm_error, py::arg("device"), "Reads and clears the products' error word of a device.");
+    o.def("gemm_error", [](int64_t device) {
+        return take_error(torch::Device(torch::kCUDA, static_cast<c10::DeviceIndex>(device)), nullptr);
+    }, py::arg("device"), "Reads and clears the products' error word of a device.");
+    o.def("take_error", [](const torch::Tensor& error) {
+        require(error.is_cuda(), "error must be a CUDA tensor");
+        return take_error(error.device(), error_word(error, error.device()));
+    }, py::arg("error"), "Reads and clears an error word of its caller's own.");
 }

@@ -605,7 +605,7 @@ void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream) {
     p.a = args;
     p.k_blocks = (args.k + kBK - 1) / kBK;
     p.nb = (args.n + 127) / 128;
-    p.error = gemm_error_word();
+    p.error = args.error ? args.error : gemm_error_word();
     const Choice c = choose(args, p.k_blocks);
     if (c.row_chunk) launch_few_rows(p, c.row_chunk, c.split, stream);
     else if (!args.swiglu) launch<kEpiStore>(p, stream);

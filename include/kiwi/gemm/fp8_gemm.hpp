@@ -39,6 +39,8 @@ struct Fp8GemmArgs {
     bool feeds_next;
     bool follows;
     bool zero_tail;           // rows past the last group's are set to zero (else left as they were)
+    uint32_t* error;          // device word that errors are reported in (bits are set, never cleared), or null:
+                              // gemm_error_word()
 };
 
 void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream);
@@ -49,8 +51,9 @@ void fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream);
 void quant_fp8_blocks(const __nv_bfloat16* w, int64_t ld, int64_t rows, int64_t cols, uint8_t* codes, float* scales,
                       cudaStream_t stream);
 
-/// The current device's error word of fp8_gemm and grouped_linear (bits in
-/// group_table.cuh).  Sticky until cleared.
+/// The current device's error word of fp8_gemm (where a call brings none of its
+/// own) and grouped_linear: one for all callers, bits in group_table.cuh, sticky
+/// until cleared.
 uint32_t* gemm_error_word();
 
 /// *out = the error word's bits, which are cleared in the same step: a bit that a

@@ -171,6 +171,11 @@ def expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale=N
     """The experts' SwiGLU FFN in FP8: ``row_scale * (quant(swiglu(x . w13^T)) . w2^T)``
     for expert-sorted rows ``x`` [rows, H], ``w13`` [E * 2F, H] (gate and up
     interleaved) and ``w2`` [E * H, F]; bf16 [rows, H].  Two launches."""
+    return _expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale, out, None)
+
+
+def _expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale, out, error):
+    """expert_ffn_fp8 with an error word (int32 [1] on the device) of the caller's own, or None."""
     counts = _as_counts(counts, x.device)
     if not x.is_cuda:
         e = counts.numel()
@@ -179,7 +184,7 @@ def expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale=N
             raise ValueError("w13 must be [E * 2F, H] and w2 [E * H, F]")
         h, hs = grouped_fp8_swiglu(x, x_scale, w13, w13_scale, counts)
         return grouped_fp8_gemm(h, hs, w2, w2_scale, counts, out, False, row_scale)
-    return _native_ops().expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale, out)
+    return _native_ops().expert_ffn_fp8(x, x_scale, w13, w13_scale, w2, w2_scale, counts, row_scale, out, error)
 
 
 def quant_fp8_weights(w):
@@ -204,11 +209,16 @@ def quant_fp8_weights(w):
 def check_gemm(device=None):
     """Raises RuntimeError if a product of this module or of
     :mod:`kiwi_b200.ops.grouped_linear` on ``device`` (the current one) reported
-    an error since the last check (synchronises the current stream)."""
+    an error since the last check (synchronises the current stream).  There is one
+    error word a device for all callers of these functions, and a check clears it
+    for all; an :class:`kiwi_b200.ops.ExpertFFN` has its own."""
     dev = torch.cuda.current_device() if device is None else torch.device(device).index
     if dev is None:
         dev = torch.cuda.current_device()
-    e = _native_ops().gemm_error(dev)
+    _raise_error(_native_ops().gemm_error(dev))
+
+
+def _raise_error(e):
     if e:
         what = [n for b, n in ((1, "a wait ran out"), (2, "counts negative or past the rows")) if e & b]
         raise RuntimeError("expert products: " + " and ".join(what))

@@ -192,6 +192,7 @@ class ExpertFFN:
 
             self.w13, self.w13_scale = quant_fp8_weights(w13)
             self.w2, self.w2_scale = quant_fp8_weights(w2)
+            self._error = torch.zeros(1, dtype=torch.int32, device=dev)
             return
         self._h = torch.zeros(rows, ffn, dtype=torch.bfloat16, device=dev)
         self.gemm1 = GroupedGemm(self._a, w13, e, b_layout=weight_layout)
@@ -204,7 +205,7 @@ class ExpertFFN:
 
     def __call__(self, counts, row_scale=None, rows=None):
         if self.weight_format == "fp8":
-            from .fp8_gemm import expert_ffn_fp8
+            from .fp8_gemm import _expert_ffn_fp8
             from .quant import quant_fp8
 
             codes, scales = quant_fp8(self._a) if rows is None else rows
@@ -212,8 +213,8 @@ class ExpertFFN:
             if n > self._y.shape[0]:
                 raise ValueError(f"{n} rows for an op of {self.max_rows}")
             y = self._y[:n]
-            expert_ffn_fp8(codes, scales, self.w13, self.w13_scale, self.w2, self.w2_scale, counts,
-                           row_scale=None if row_scale is None else row_scale[:n], out=y)
+            _expert_ffn_fp8(codes, scales, self.w13, self.w13_scale, self.w2, self.w2_scale, counts,
+                            None if row_scale is None else row_scale[:n], y, self._error)
             return y
         if rows is not None:
             raise ValueError("FP8 rows need weight_format='fp8'")
@@ -222,11 +223,13 @@ class ExpertFFN:
         return self._y
 
     def check(self):
+        """Raises RuntimeError if a call of this object reported an error
+        (synchronises).  With FP8 weights the check clears it."""
         if self.weight_format == "fp8":
             if self._a.is_cuda:
-                from .fp8_gemm import check_gemm
+                from .fp8_gemm import _native_ops, _raise_error
 
-                check_gemm(self._a.device)
+                _raise_error(_native_ops().take_error(self._error))
             return
         self.gemm1.check()
         self.gemm2.check()

@@ -145,3 +145,21 @@ def test_error_word_is_taken_in_one_step():
     names = [e.name for e in p.events()]
     assert any("take_error" in n for n in names) and not any("emset" in n for n in names), names
     ops.check_gemm()
+
+
+def _ffn(seed):
+    g = _gen(seed)
+    w13, w2 = ((torch.randn(2 * 256, k, generator=g, device="cuda") * 0.02).bfloat16() for k in (256, 128))
+    return ops.ExpertFFN(w13, w2, 2, 8, weight_format="fp8")
+
+
+def test_each_ffn_reports_its_own_errors():
+    a, b = _ffn(1), _ffn(2)
+    good, bad = (torch.tensor(c, dtype=torch.int32, device="cuda") for c in ([4, 4], [4, 5]))
+    ops.check_gemm()
+    a(bad), b(good)
+    b.check()
+    ops.check_gemm()  # an object's errors are its own
+    with pytest.raises(RuntimeError, match="counts"):
+        a.check()
+    a.check()
