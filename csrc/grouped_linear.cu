@@ -428,7 +428,7 @@ void check(const GroupedLinearArgs& a) {
     if (a.rows < 0 || a.rows > INT32_MAX - 256 || static_cast<int64_t>(a.num_groups) * a.n > INT32_MAX - 256) {
         throw kiwi::error("grouped_linear: more than 2^31 rows");
     }
-    if (a.ldo % 8 || reinterpret_cast<uintptr_t>(a.out) % 16) {
+    if (a.ldo * (a.out_fp32 ? 4 : 2) % 16 || reinterpret_cast<uintptr_t>(a.out) % 16) {
         throw kiwi::error("grouped_linear: the result's rows must start on 16-byte boundaries");
     }
 }

@@ -10,7 +10,7 @@ namespace kiwi::gemm {
 
 /// Rows of x [rows, k], y and dy [rows, n] belong to groups of counts[g]
 /// consecutive rows; w is [num_groups * n, k].  n and k are multiples of 64;
-/// row strides (elements) of multiples of 8, bases on 16-byte boundaries.
+/// rows start on 16-byte boundaries (bases and row strides of multiples of 16 bytes).
 struct GroupedLinearArgs {
     const __nv_bfloat16* x;   // forward, wgrad
     int64_t ldx;

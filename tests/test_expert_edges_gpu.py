@@ -163,3 +163,16 @@ def test_each_ffn_reports_its_own_errors():
     with pytest.raises(RuntimeError, match="counts"):
         a.check()
     a.check()
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_weight_gradient_into_fp32_rows_of_four(accumulate):
+    g = _gen(5)
+    x, dy = (torch.randn(70, 64, generator=g, device="cuda").bfloat16() for _ in range(2))
+    cnt = torch.tensor([70], dtype=torch.int32, device="cuda")
+    wide = torch.full((64, 68), 2.0, device="cuda")
+    ops.grouped_linear_wgrad(dy, x, cnt, out=wide[:, :64], accumulate=accumulate)
+    ref = dy.double().T @ x.double()
+    bound = 70 * F32 * (dy.double().abs().T @ x.double().abs()) + 4 * F32 * (ref.abs() + 2)
+    assert bool(((wide[:, :64].double() - ref - (2 if accumulate else 0)).abs() <= bound).all())
+    assert bool((wide[:, 64:] == 2).all())
