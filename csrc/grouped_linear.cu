@@ -420,7 +420,7 @@ CUtensorMap bf16_map(const __nv_bfloat16* ptr, int64_t rows, int64_t cols, int64
     return make_tmap_2d(ptr, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, cols, ld * 2, box_rows, kBK);
 }
 
-void check(const GroupedLinearArgs& a) {
+void check(const GroupedLinearArgs& a, int out_bytes) {
     if (a.num_groups < 1 || a.num_groups > kMaxGroups) throw kiwi::error("grouped_linear: 1..1024 groups");
     if (a.n < 64 || a.n % 64 || a.k < 64 || a.k % 64) throw kiwi::error("grouped_linear: N and K must be multiples of 64");
     if (a.k > INT32_MAX - 256) throw kiwi::error("grouped_linear: K must be below 2^31 - 256");
@@ -428,7 +428,7 @@ void check(const GroupedLinearArgs& a) {
     if (a.rows < 0 || a.rows > INT32_MAX - 256 || static_cast<int64_t>(a.num_groups) * a.n > INT32_MAX - 256) {
         throw kiwi::error("grouped_linear: more than 2^31 rows");
     }
-    if (a.ldo * (a.out_fp32 ? 4 : 2) % 16 || reinterpret_cast<uintptr_t>(a.out) % 16) {
+    if (a.ldo * out_bytes % 16 || reinterpret_cast<uintptr_t>(a.out) % 16) {
         throw kiwi::error("grouped_linear: the result's rows must start on 16-byte boundaries");
     }
 }
@@ -459,7 +459,7 @@ int64_t most_row_blocks(const GroupedLinearArgs& a) {
 }  // namespace
 
 void grouped_linear_forward(const GroupedLinearArgs& a, cudaStream_t stream) {
-    check(a);
+    check(a, 2);
     if (a.rows == 0) return;
     Params p{a, a.n, a.k / kBK, gemm_error_word()};
     launch<kForward, __nv_bfloat16>(bf16_map(a.w, static_cast<int64_t>(a.num_groups) * a.n, a.k, a.ldw, 128),
@@ -468,7 +468,7 @@ void grouped_linear_forward(const GroupedLinearArgs& a, cudaStream_t stream) {
 }
 
 void grouped_linear_dgrad(const GroupedLinearArgs& a, cudaStream_t stream) {
-    check(a);
+    check(a, 2);
     if (a.rows == 0) return;
     Params p{a, a.k, a.n / kBK, gemm_error_word()};
     launch<kDgrad, __nv_bfloat16>(bf16_map(a.w, static_cast<int64_t>(a.num_groups) * a.n, a.k, a.ldw, 64),
@@ -477,7 +477,7 @@ void grouped_linear_dgrad(const GroupedLinearArgs& a, cudaStream_t stream) {
 }
 
 void grouped_linear_wgrad(const GroupedLinearArgs& a, cudaStream_t stream) {
-    check(a);
+    check(a, a.out_fp32 ? 4 : 2);
     Params p{a, a.n, 0, gemm_error_word()};
     const int64_t tiles = static_cast<int64_t>(a.num_groups) * ((a.n + kBM - 1) / kBM) * ((a.k + kBN - 1) / kBN);
     if (tiles > INT32_MAX) throw kiwi::error("grouped_linear: result too large");

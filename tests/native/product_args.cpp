@@ -83,6 +83,11 @@ int main() {
     fp8("fp8 large k", [](auto& a) { a.k = INT32_MAX - 15; });
     linear("forward large k", kiwi::gemm::grouped_linear_forward, [](auto& a) { a.k = INT32_MAX - 63; });
     linear("dgrad large k", kiwi::gemm::grouped_linear_dgrad, [](auto& a) { a.k = INT32_MAX - 63; });
+    linear("forward unaligned rows", kiwi::gemm::grouped_linear_forward, [](auto& a) {
+        a.out_fp32 = true;  // of no effect: y is bf16
+        a.ldo = 260;
+    });
+    linear("wgrad unaligned rows", kiwi::gemm::grouped_linear_wgrad, [](auto& a) { a.ldo = 260; });
     linear("wgrad large k", kiwi::gemm::grouped_linear_wgrad, [](auto& a) { a.k = INT32_MAX - 63; });
     return 0;
 }

@@ -44,6 +44,8 @@ def refusals(tmp_path_factory):
     ("forward large k", "2^31"),
     ("dgrad large k", "2^31"),
     ("wgrad large k", "2^31"),
+    ("forward unaligned rows", "16-byte boundaries"),
+    ("wgrad unaligned rows", "16-byte boundaries"),
 ])
 def test_refused_before_a_device_is_touched(refusals, case, words):
     assert words in refusals[case], refusals[case]
