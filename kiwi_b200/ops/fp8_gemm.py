@@ -88,12 +88,15 @@ def _check(a, a_scale, b, b_scale, counts, out, swiglu, row_scale):
 
 
 def _as_counts(counts, device):
-    """int32 row counts on the rows' device (a host list is copied there)."""
+    """int32 row counts on the rows' device (a host list is copied there).  What
+    32 bits cannot hold is saturated to a count that is reported, not wrapped."""
     if torch.is_tensor(counts) and counts.dtype == torch.int32 and counts.device == device:
         return counts
     counts = torch.as_tensor(counts)
     if counts.is_floating_point() and counts.numel():
         raise ValueError("counts must be whole numbers")
+    if counts.element_size() > 2 and counts.dtype != torch.int32:
+        counts = counts.to(torch.int64).clamp(-1, 2 ** 31 - 1)
     return counts.to(device=device, dtype=torch.int32)
 
 

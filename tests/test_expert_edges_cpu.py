@@ -93,3 +93,24 @@ def test_rows_too_long_for_32_bits():
     x = torch.empty(64, 2 ** 31 - 64, dtype=torch.bfloat16, device="meta")
     with pytest.raises(ValueError, match="2\\^31"):
         ops.grouped_linear(x, x, torch.tensor([64]))
+
+
+@pytest.mark.parametrize("counts", [[2 ** 32 + 4], [2 ** 31], [-2 ** 32 + 4], [2 ** 32, 4], [2 ** 62 + 2, 2]])
+def test_counts_past_32_bits(counts):
+    """They were wrapped into 32 bits, 2^32 + 4 into 4."""
+    e = len(counts)
+    a, s = torch.zeros(8, 128).to(torch.float8_e4m3fn), torch.ones(8, 1)
+    b, sb = torch.zeros(e * 128, 128).to(torch.float8_e4m3fn), torch.ones(e, 1)
+    x, w = torch.zeros(8, 64).bfloat16(), torch.zeros(e * 64, 64).bfloat16()
+    for c in (counts, torch.tensor(counts)):
+        with pytest.raises(ValueError, match="counts"):
+            ops.grouped_fp8_gemm(a, s, b, sb, c)
+        with pytest.raises(ValueError, match="counts"):
+            ops.grouped_linear(x, w, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16, torch.uint8])
+def test_counts_of_every_whole_type(dtype):
+    x, w = torch.randn(8, 64).bfloat16(), torch.randn(128, 64).bfloat16()
+    want = ops.grouped_linear(x, w, [3, 5])
+    assert torch.equal(ops.grouped_linear(x, w, torch.tensor([3, 5], dtype=dtype)), want)

@@ -176,3 +176,17 @@ def test_weight_gradient_into_fp32_rows_of_four(accumulate):
     bound = 70 * F32 * (dy.double().abs().T @ x.double().abs()) + 4 * F32 * (ref.abs() + 2)
     assert bool(((wide[:, :64].double() - ref - (2 if accumulate else 0)).abs() <= bound).all())
     assert bool((wide[:, 64:] == 2).all())
+
+
+@pytest.mark.parametrize("counts", [[2 ** 32 + 4], [2 ** 31], [-2 ** 32 + 4]])
+def test_counts_past_32_bits_are_reported(counts):
+    g = _gen(4)
+    a, sa, _ = _fp8(g, 8, 128)
+    b, sb, _ = _fp8_weights(g, 256, 128)
+    x, w = torch.zeros(8, 64, device="cuda").bfloat16(), torch.zeros(64, 64, device="cuda").bfloat16()
+    cnt = torch.tensor(counts, device="cuda")
+    ops.check_gemm()
+    for f in (lambda: ops.grouped_fp8_gemm(a, sa, b, sb, cnt), lambda: ops.grouped_linear(x, w, cnt)):
+        f()
+        with pytest.raises(RuntimeError, match="counts"):
+            ops.check_gemm()
