@@ -109,11 +109,23 @@ unsigned blocks_for(int64_t rows) {
     return static_cast<unsigned>(b);
 }
 
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+void check(const __nv_bfloat16* y, int64_t ldy, const __nv_bfloat16* out, int ffn) {
+    if (!y || !out) throw kiwi::error("swiglu: missing input or output");
+    if (ffn < 128 || ffn % 128 || ffn > (INT32_MAX - 256) / 2) {
+        throw kiwi::error("swiglu: the hidden columns must be a positive multiple of 128, in all fewer than 2^30");
+    }
+    if (ldy < 2 * static_cast<int64_t>(ffn)) throw kiwi::error("swiglu: row stride below the rows' length");
+    if (!aligned16(y) || !aligned16(out) || ldy % 8) throw kiwi::error("swiglu: rows must start on 16-byte boundaries");
+}
+
 }  // namespace
 
 void swiglu_forward(const __nv_bfloat16* y, int64_t ldy, const float* row_scale, __nv_bfloat16* h, int64_t rows,
                     int ffn, cudaStream_t s) {
     if (rows <= 0) return;
+    check(y, ldy, h, ffn);
     swiglu_forward_kernel<<<blocks_for(rows), kThreads, 0, s>>>(y, ldy, row_scale, h, rows, ffn);
     KIWI_CUDA_CHECK(cudaGetLastError());
 }
@@ -122,6 +134,10 @@ void swiglu_backward(const __nv_bfloat16* dh, int64_t lddh, const __nv_bfloat16*
                      const float* row_scale, __nv_bfloat16* dy, float* drow_scale, int64_t rows, int ffn,
                      cudaStream_t s) {
     if (rows <= 0) return;
+    check(y, ldy, dy, ffn);
+    if (!dh) throw kiwi::error("swiglu: missing dh");
+    if (lddh < ffn) throw kiwi::error("swiglu: dh's row stride below its rows' length");
+    if (!aligned16(dh) || lddh % 8) throw kiwi::error("swiglu: dh's rows must start on 16-byte boundaries");
     swiglu_backward_kernel<<<blocks_for(rows), kThreads, 0, s>>>(dh, lddh, y, ldy, row_scale, dy, drow_scale, rows,
                                                                  ffn);
     KIWI_CUDA_CHECK(cudaGetLastError());

@@ -8,9 +8,10 @@
 
 namespace kiwi::ops {
 
-/// h[r, j] = row_scale[r] * silu(gate) * up for y [rows, 2 * ffn] (row stride ldy,
-/// a multiple of 8, 16-byte aligned) whose columns come in blocks of 128 gate and
-/// 128 up columns; h [rows, ffn] contiguous.  row_scale may be null (1).
+/// h[r, j] = row_scale[r] * silu(gate) * up for y [rows, 2 * ffn] whose columns
+/// come in blocks of 128 gate and 128 up columns (ffn is a multiple of 128);
+/// h [rows, ffn] contiguous.  Row strides (ldy, lddh) are multiples of 8, all
+/// bases on 16-byte boundaries.  row_scale may be null (1).
 void swiglu_forward(const __nv_bfloat16* y, int64_t ldy, const float* row_scale, __nv_bfloat16* h, int64_t rows,
                     int ffn, cudaStream_t s);
 

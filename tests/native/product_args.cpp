@@ -1,15 +1,17 @@
 // Argument checks of the C++ entries of the experts' products (no GPU needed):
 // prints "case: message" for each refused call.  No pointer passed here is ever
-// dereferenced, and nothing can be launched: the number of SMs, which every
-// launch asks for first, is refused by this file.
+// dereferenced: each call fails a check, and a product that passed them all
+// would ask this file for the number of SMs before its launch.
 #include <cstdint>
 #include <cstdio>
 #include <functional>
+#include <string>
 
 #include "kiwi/common.hpp"
 #include "kiwi/gemm/fp8_gemm.hpp"
 #include "kiwi/gemm/grouped_gemm.hpp"
 #include "kiwi/gemm/grouped_linear.hpp"
+#include "kiwi/ops/swiglu.hpp"
 
 namespace kiwi::gemm {
 int num_sms() { throw kiwi::error("accepted"); }
@@ -73,6 +75,17 @@ void linear(const char* name, void (*entry)(const kiwi::gemm::GroupedLinearArgs&
     report(name, [&] { entry(a, nullptr); });
 }
 
+/// Both directions of SwiGLU; the backward's dh has y's base and a row stride to match.
+void swiglu(const char* name, uintptr_t y, int64_t ldy, uintptr_t out, int ffn) {
+    report(name, [&] {
+        kiwi::ops::swiglu_forward(at<__nv_bfloat16>(y), ldy, nullptr, at<__nv_bfloat16>(out), 8, ffn, nullptr);
+    });
+    report((std::string(name) + " backward").c_str(), [&] {
+        kiwi::ops::swiglu_backward(at<__nv_bfloat16>(y), ldy, at<__nv_bfloat16>(y), ldy, nullptr,
+                                   at<__nv_bfloat16>(out), nullptr, 8, ffn, nullptr);
+    });
+}
+
 }  // namespace
 
 int main() {
@@ -89,5 +102,13 @@ int main() {
     });
     linear("wgrad unaligned rows", kiwi::gemm::grouped_linear_wgrad, [](auto& a) { a.ldo = 260; });
     linear("wgrad large k", kiwi::gemm::grouped_linear_wgrad, [](auto& a) { a.k = INT32_MAX - 63; });
+    swiglu("swiglu columns", kBase, 512, kBase, 192);
+    swiglu("swiglu no columns", kBase, 512, kBase, 0);
+    swiglu("swiglu row stride", kBase, 516, kBase, 256);
+    swiglu("swiglu short rows", kBase, 504, kBase, 256);
+    swiglu("swiglu input base", kBase + 8, 512, kBase, 256);
+    swiglu("swiglu output base", kBase, 512, kBase + 2, 256);
+    swiglu("swiglu missing input", 0, 512, kBase, 256);
+    swiglu("swiglu missing output", kBase, 512, 0, 256);
     return 0;
 }

@@ -9,7 +9,7 @@ import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 NVCC = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-SOURCES = ["csrc/fp8_gemm.cu", "csrc/fp8_few_rows.cu", "csrc/grouped_linear.cu", "csrc/tensor_map.cpp", "src/p2p/driver.cpp",
+SOURCES = ["csrc/fp8_gemm.cu", "csrc/fp8_few_rows.cu", "csrc/grouped_linear.cu", "csrc/swiglu_gpu.cu", "csrc/tensor_map.cpp", "src/p2p/driver.cpp",
            "tests/native/product_args.cpp"]
 
 
@@ -46,6 +46,16 @@ def refusals(tmp_path_factory):
     ("wgrad large k", "2^31"),
     ("forward unaligned rows", "16-byte boundaries"),
     ("wgrad unaligned rows", "16-byte boundaries"),
+    ("swiglu columns", "multiple of 128"),
+    ("swiglu no columns", "multiple of 128"),
+    ("swiglu row stride", "16-byte boundaries"),
+    ("swiglu short rows", "row stride"),
+    ("swiglu input base", "16-byte boundaries"),
+    ("swiglu output base", "16-byte boundaries"),
+    ("swiglu missing input", "missing"),
+    ("swiglu missing output", "missing"),
 ])
 def test_refused_before_a_device_is_touched(refusals, case, words):
     assert words in refusals[case], refusals[case]
+    if case.startswith("swiglu"):
+        assert words in refusals[case + " backward"], refusals[case + " backward"]
