@@ -340,7 +340,7 @@ torch::Tensor linear_wgrad_py(torch::Tensor dy, torch::Tensor x, torch::Tensor c
 void check_swiglu(const torch::Tensor& y, const OptTensor& row_scale) {
     check_bf16_rows(y, y.device(), "y");
     require(y.size(1) >= 256 && y.size(1) % 256 == 0, "y must have a multiple of 256 columns (128 gate, 128 up, ...)");
-    require(y.size(1) < (int64_t{1} << 31), "fewer than 2^31 columns");
+    require(y.size(1) <= INT32_MAX - 256, "y must have fewer than 2^31 - 256 columns");
     check_row_scale(row_scale, y.size(0), y.device());
 }
 

@@ -90,6 +90,8 @@ def test_rows_too_long_for_32_bits():
     x = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(64, 2 ** 31 - 64)
     with pytest.raises(ValueError, match="2\\^31"):
         ops.grouped_linear(x, x, torch.tensor([64], dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.swiglu(x[:1, :1].expand(1, 2 ** 31 - 256))
 
 
 def test_ffn_refuses_an_out_over_its_row_scale_before_it_launches():
