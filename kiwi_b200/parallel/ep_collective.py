@@ -394,6 +394,8 @@ class CollectiveMoE:
         self._scale[:p].copy_(rw[r, s])
         if fp8_rows:
             y = self.experts(counts, self._scale, rows=(rows[r], scales[r]))
+        elif self.experts.weight_format == "fp8":  # these rows alone, not the experts' whole buffer
+            y = self.experts(counts, self._scale, rows=quant_fp8(rows[r].to(torch.bfloat16)))
         else:
             self.experts.input_buffer()[:p].copy_(rows[r])
             y = self.experts(counts, self._scale)

@@ -114,3 +114,22 @@ def test_counts_of_every_whole_type(dtype):
     x, w = torch.randn(8, 64).bfloat16(), torch.randn(128, 64).bfloat16()
     want = ops.grouped_linear(x, w, [3, 5])
     assert torch.equal(ops.grouped_linear(x, w, torch.tensor([3, 5], dtype=dtype)), want)
+
+
+@pytest.mark.parametrize("quant", ["none", "fp8", "nvfp4"])
+def test_collective_layer_gives_its_fp8_experts_the_rows_it_has(quant, monkeypatch):
+    """The experts' buffer is sized for the worst case; a step works on the rows
+    that arrived, not on all of it."""
+    from kiwi_b200.parallel.ep_collective import CollectiveMoE
+
+    cfg = moe.MoEConfig(hidden=256, ffn=128, num_experts=3, topk=2, tokens_per_rank=50, quant=quant, name="t")
+    layer = CollectiveMoE(cfg, device="cpu", weight_format="fp8")
+    seen = []
+    call = ops.ExpertFFN.__call__
+    monkeypatch.setattr(ops.ExpertFFN, "__call__", lambda self, counts, scale=None, rows=None: (
+        seen.append((int(counts.sum()), self.max_rows if rows is None else len(rows[0]))), call(self, counts, scale, rows))[1])
+    for tokens in (7, 0, 50):
+        x, logits = moe.synthetic_inputs(cfg, 0, "cpu", tokens=tokens)
+        out = layer(x, logits)
+        assert tuple(out.shape) == (tokens, 256) and bool(torch.isfinite(out).all())
+    assert seen == [(14, 14), (0, 0), (100, 100)]

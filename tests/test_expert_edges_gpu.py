@@ -192,3 +192,24 @@ def test_counts_past_32_bits_are_reported(counts):
         f()
         with pytest.raises(RuntimeError, match="counts"):
             ops.check_gemm()
+
+
+@pytest.mark.parametrize("quant", ["none", "fp8", "nvfp4"])
+def test_collective_layer_with_fp8_experts_and_few_or_no_tokens(quant):
+    """Tokens are independent of one another but for the order of an fp32 sum,
+    which the number of rows decides: a few tokens come out as they do among
+    others, to a bf16 rounding of each expert's row and of their sum, and to the
+    neighbouring e4m3 code (2^-3 of a value) of hidden values on a border, of
+    which the norm sees few."""
+    from kiwi_b200.models import moe
+    from kiwi_b200.parallel.ep_collective import CollectiveMoE
+
+    cfg = moe.MoEConfig(hidden=512, ffn=256, num_experts=4, topk=2, tokens_per_rank=600, quant=quant, name="t")
+    layer = CollectiveMoE(cfg, weight_format="fp8")
+    x, logits = moe.synthetic_inputs(cfg, 0, "cuda", tokens=600)
+    full = layer(x, logits)
+    for t in (0, 1, 37):
+        out = layer(x[:t], logits[:t])
+        assert tuple(out.shape) == (t, 512) and bool(torch.isfinite(out).all())
+        assert (out.float() - full[:t].float()).norm() <= 2 * BF16 * full[:t].float().norm()
+    layer.check()
