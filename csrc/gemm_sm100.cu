@@ -29,7 +29,7 @@
 #include "kiwi/ep/quant.cuh"
 #include "kiwi/ep/debug_timing.hpp"
 #include "kiwi/gemm/grouped_gemm.hpp"
-#include "kiwi/p2p/driver.hpp"
+#include "kiwi/gemm/tensor_map.hpp"
 #include "kiwi/p2p/heap.hpp"
 #include "kiwi/sm100.cuh"
 
@@ -888,29 +888,8 @@ __global__ void build_split_schedule_kernel(const int32_t* counts, int num_group
 }  // namespace
 
 CUtensorMap make_tmap_bf16_2d(const void* ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_k) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    if (!encode) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        KIWI_CUDA_CHECK(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q));
-        if (q != cudaDriverEntryPointSuccess || !fn) throw kiwi::error("cuTensorMapEncodeTiled unavailable");
-        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0 || (cols * 2) % 16 != 0) {
-        throw kiwi::error("make_tmap_bf16_2d: base and row stride must be 16-byte aligned");
-    }
-    CUtensorMap m;
-    const cuuint64_t dims[2] = {cols, rows};
-    const cuuint64_t strides[1] = {cols * 2};
     if (box_k != 64 && box_k != 32) throw kiwi::error("make_tmap_bf16_2d: box_k must be 64 or 32");
-    const cuuint32_t box[2] = {box_k, box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              box_k == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    p2p::check_cu(r, "cuTensorMapEncodeTiled");
-    return m;
+    return make_tmap_2d(ptr, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, cols, cols * 2, box_rows, box_k);
 }
 
 void build_schedule(const int32_t* counts, int num_groups, int n, int bn, int32_t* offsets, int32_t* tile_prefix,

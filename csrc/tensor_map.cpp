@@ -25,7 +25,8 @@ CUtensorMap make_tmap_2d(const void* ptr, CUtensorMapDataType type, int elem, ui
     if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0 || ld_bytes % 16 != 0) {
         throw kiwi::error("make_tmap_2d: base and row stride must be multiples of 16 bytes");
     }
-    if (box_cols * elem != 128) throw kiwi::error("make_tmap_2d: box rows must be 128 bytes");
+    const uint32_t box_bytes = box_cols * static_cast<uint32_t>(elem);
+    if (box_bytes != 128 && box_bytes != 64) throw kiwi::error("make_tmap_2d: box rows must be 128 or 64 bytes");
     // A thread that has made no runtime call yet, such as autograd's worker, has
     // no current context, and the driver call below does not bind one.
     static thread_local bool bound = false;
@@ -41,7 +42,8 @@ CUtensorMap make_tmap_2d(const void* ptr, CUtensorMapDataType type, int elem, ui
     const cuuint32_t box[2] = {box_cols, box_rows};
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = encode(&m, type, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     p2p::check_cu(r, "cuTensorMapEncodeTiled");
     return m;

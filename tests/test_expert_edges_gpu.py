@@ -213,3 +213,25 @@ def test_collective_layer_with_fp8_experts_and_few_or_no_tokens(quant):
         assert tuple(out.shape) == (t, 512) and bool(torch.isfinite(out).all())
         assert (out.float() - full[:t].float()).norm() <= 2 * BF16 * full[:t].float().norm()
     layer.check()
+
+
+def test_products_in_a_thread_of_their_own():
+    """Tensor maps are built by the driver, which needs a context that a new
+    thread may not have bound yet."""
+    import threading
+
+    g = _gen(8)
+    a, sa, _ = _fp8(g, 40, 256)
+    b, sb, _ = _fp8_weights(g, 256, 256)
+    x, w = (torch.randn(r, 256, generator=g, device="cuda").bfloat16() for r in (40, 256))
+    cnt = torch.tensor([40], dtype=torch.int32, device="cuda")
+    out = torch.empty(40, 256, dtype=torch.bfloat16, device="cuda")
+    calls = [lambda: ops.fp8_gemm(a, sa, b, sb, out=out).clone(), lambda: ops.grouped_linear(x, w, cnt, out=out).clone(),
+             lambda: ops.GroupedGemm(x, w, 1)(cnt, out)[:40].clone()]
+    for f in calls:
+        want, got = f(), []
+        t = threading.Thread(target=lambda: got.append(f()))
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert len(got) == 1 and torch.equal(got[0], want)
