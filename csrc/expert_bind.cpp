@@ -436,6 +436,7 @@ struct SwiGLU : torch::autograd::Function<SwiGLU> {
 
 /// Reads and clears an error word, or a device's (waits for the current stream).
 int64_t take_error(const torch::Device& dev, uint32_t* word) {
+    py::gil_scoped_release nogil;  // what it waits for may be waiting for a callback in Python
     const c10::cuda::CUDAGuard guard(dev);
     const torch::Tensor bits = torch::empty({1}, torch::dtype(torch::kInt32).device(dev));
     gemm::take_error(word ? word : gemm::gemm_error_word(), reinterpret_cast<uint32_t*>(bits.data_ptr<int32_t>()), cur_stream());

@@ -235,3 +235,30 @@ def test_products_in_a_thread_of_their_own():
         t.join()
         torch.cuda.synchronize()
         assert len(got) == 1 and torch.equal(got[0], want)
+
+
+def test_a_check_lets_other_threads_run_while_it_waits():
+    """A kernel ahead of it on the stream may be waiting for a callback in Python."""
+    import threading
+    import time
+
+    ops.check_gemm()
+    stop, ticks = threading.Event(), []
+
+    def tick():
+        while not stop.is_set():
+            ticks.append(time.perf_counter())
+            time.sleep(1e-3)
+
+    t = threading.Thread(target=tick)
+    t.start()
+    try:
+        torch.cuda._sleep(1_000_000_000)  # half a second of a busy GPU
+        begin = time.perf_counter()
+        ops.check_gemm()
+        end = time.perf_counter()
+    finally:
+        stop.set()
+        t.join()
+    assert end - begin > 0.1
+    assert sum(begin < x < end for x in ticks) > 10
