@@ -27,7 +27,7 @@
 //   warps 0..7   drain: TMEM lane quadrant = warp % 4, weight block = warp / 4;
 //                then a token's 256 columns a warp
 //   warp 8       TMA producer      warp 9  TMEM owner and MMA issuer
-//   warps 10, 11 scales: sa * sb of every token and weight block, a block ahead
+//   warp 10      scales: sa * sb of every token and weight block, a block ahead
 // Every wait is bounded; one that runs out sets the error word, and the CTA
 // drains its loads, frees its TMEM and leaves.
 #include <cuda.h>

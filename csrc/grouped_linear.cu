@@ -30,9 +30,10 @@
 // onto a barrier of its own, clears the rows and arrives at the leader's.  A
 // group without rows gets zeros.
 //
-// Bound by the power cap where groups are long: 1.35 to 1.53 PFLOP/s on even
-// groups of 512 to 2048 rows in bursts (0.81 to 0.92 of the measured rate),
-// 1.2 in a long run at 1.15 GHz; wgrad, where groups are short, by writing dw:
+// Bound where groups are long by the tensor cores and, in long runs, in part by
+// the power cap: 1.35 to 1.53 PFLOP/s on even groups of 512 to 2048 rows in bursts
+// (0.81 to 0.92 of the measured rate), 1.2 in a long run at 1.15 GHz, where a
+// plain library product holds 1.39; wgrad, where groups are short, by writing dw:
 // 3.4 to 3.6 TB/s of the 3.95 that a fill reaches.  Measured on one B200, n x k =
 // 4096 x 7168, 16384 rows over 32 groups: even groups forward 702 us, dgrad 711,
 // wgrad 857; uneven ones (Zipf 0.3) 842, 792, 990, and in a long run of all three

@@ -1,8 +1,10 @@
 // The tile schedule of a grouped product, built by every CTA in its own shared
 // memory from the groups' row counts on the device: no schedule launch before
 // the product, no host synchronisation, no workspace that two launches could
-// share.  One read of at most 4 KB of counts and a warp scan cost about a
-// microsecond at 1024 groups and less than the barrier set-up at 32.
+// share.  All warps of the CTA scan the counts, 32 groups at a time.  A launch
+// whose groups are all empty takes 3.0 us with one group, 3.1 to 3.4 with 32 to
+// 256 and 4.9 (bf16 product: 5.8) with 1024, in graphs on one B200: the table is
+// 2 to 3 us of it at 1024 groups and nothing to speak of below 256.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -164,9 +164,11 @@ class ExpertFFN:
     scales (:func:`kiwi_b200.ops.quant_fp8_weights`; half the memory, row-major
     whatever ``weight_layout``) and runs both products in FP8
     (:func:`kiwi_b200.ops.expert_ffn_fp8`).  H and F are then multiples of 128,
-    and each call quantises the input buffer's rows, or takes rows that are FP8
-    already: ``ffn(counts, row_scale, rows=(codes, scales))`` with 1 x 128 scales,
-    as the FP8 dispatch delivers them, returns as many rows as those have."""
+    and each call quantises the whole input buffer, all ``max_rows`` rows of it
+    whatever the counts say, or takes rows that are FP8 already: ``ffn(counts,
+    row_scale, rows=(codes, scales))`` with 1 x 128 scales, as the FP8 dispatch or
+    :func:`kiwi_b200.ops.quant_fp8` delivers them, works on those and returns as
+    many rows."""
 
     def __init__(self, w13, w2, num_experts, max_rows, weight_layout="blocked", weight_format="bf16"):
         e = int(num_experts)

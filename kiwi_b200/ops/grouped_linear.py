@@ -20,15 +20,18 @@ passed in, and never read; a group without rows has a zero ``dw`` (with
 blocks of 128 gate and 128 up columns, differentiable in ``y`` and
 ``row_scale``.  A routing weight applied here is the same as one applied to the
 second product's rows, and its gradient needs no product.  ``expert_ffn`` is the
-three together: the experts' FFN for training.
+three together: the experts' FFN for training.  On CUDA tensors the sigmoid is
+made of the approximate exponential and reciprocal, which stay far below a bf16
+rounding; the fp32 gradient of ``row_scale`` is off by up to 0.30 steps of 2^-23 of
+the sum of its terms' magnitudes, with exact functions by 0.24.
 
 CUDA tensors run the sm_100a kernels on the current stream: nothing
 synchronises, and the calls can be captured into a CUDA graph (a captured
 backward needs, as in any PyTorch program, a warm-up on the capturing stream and
 leaves that no live eager graph still accumulates into).  Counts that are
 negative or add up to more than the rows are clamped and reported by
-:func:`kiwi_b200.ops.check_gemm`.  CPU tensors run the same sums in fp32.
-Gradients are once differentiable.
+:func:`kiwi_b200.ops.check_gemm` (a call without rows reports nothing).  CPU
+tensors run the same sums in fp32.  Gradients are once differentiable.
 """
 import torch
 
