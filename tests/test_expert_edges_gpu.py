@@ -145,6 +145,8 @@ def test_error_word_is_taken_in_one_step():
         with pytest.raises(RuntimeError, match="counts"):
             ops.check_gemm()
     names = [e.name for e in p.events()]
+    if not names:
+        pytest.skip("no profiler events on this machine")
     assert any("take_error" in n for n in names) and not any("emset" in n for n in names), names
     ops.check_gemm()
 
